@@ -201,6 +201,17 @@ class HipCodeGen:
         if lora:
             unit.define("CL_LORA", 1)
             unit.define("CL_R", p["R"])
+        ep = p.get("epilogue")
+        if ep:
+            # (ahead of every template that stores a product: the helper each of them calls)
+            from ..ir.families import ACTIVATIONS
+
+            for k, v in (("", 1), ("_ACT", ("none", *ACTIVATIONS).index(ep["act"])), ("_BIAS", ep["bias"]), ("_RES", ep["res"])):
+                unit.define(f"CL_EPI{k}", v)
+            for role in ("BIAS", "RES"):
+                if role in op:
+                    unit.define(f"CL_ARG_{role}", op[role])
+            unit.templates.append("epilogue.hip")
         unit.define("CL_NORM", norm)
         unit.define("CL_GAMMA", bool(norm and p.get("gamma")))
         unit.define("CL_EPS", _f(p.get("eps", 0.0)))
@@ -241,7 +252,8 @@ class HipCodeGen:
             else:
                 # the combine reads the same allocation under its `_combine` name
                 sig = [names[op["PACC_COMBINE"]]] + ([names[op["PSS_COMBINE"]]] if norm else []) \
-                    + ([names[op["PD_COMBINE"]], names[op["LB"]]] if lora else []) + outs
+                    + ([names[op["PD_COMBINE"]], names[op["LB"]]] if lora else []) \
+                    + [names[op[r]] for r in ("BIAS", "RES") if r in op] + outs
                 entry, suffix = COMBINE_ENTRY, "_COMBINE"
             unit.define("CL_CARG_PACC", op["PACC" + suffix])
             if norm:

@@ -1,0 +1,84 @@
+// ---- what follows a matrix product before it is stored: y = act(x w + bias) + residual -----------------
+//
+// The sums of the product are f32 and stay so: bias and residual are widened, the activation is taken in f32, and the result
+// is rounded to the element type once.  (A product stored in the element type, and read again by a kernel that adds and
+// activates, is rounded twice and moves 4 M N bytes more.)
+//   CL_EPI_ACT   0 none, 1 relu, 2 silu, 3 gelu, 4 gelu's tanh form     CL_EPI_BIAS  a row (1, N)     CL_EPI_RES  (M, N)
+//
+// silu(x) = x / (1 + e^-x).  The tanh form of gelu is x / 2 (1 + tanh u) = x / (1 + e^-2u), u = sqrt(2 / pi) (x + 0.044715 x^3).
+// Where e^.. overflows, the quotient is -0 and x, as the limits are.
+// gelu(x) = x / 2 erfc(-x / sqrt 2).  For z >= 0, erfc(z) = e^(-z^2) q(z), and q is a polynomial in t = 1 / (1 + 0.4 z) without a
+// constant term, fitted here to e^(z^2) erfc(z) over [0, 200] by weighted least squares: relative error 1.3e-7, with f32 arithmetic
+// 4e-7 (to f16 in its range a tenth of a rounding); erfc(-z) = 2 - erfc(z).
+CL_DEVICE float ep_exp(float x) { return fast_exp2(x * 1.4426950408889634f); }
+
+CL_DEVICE float ep_act(float x) {
+#if CL_EPI_ACT == 1
+  return x < 0.f ? 0.f : x;                 // (NaN stays NaN)
+#elif CL_EPI_ACT == 2
+  return x * fast_rcp(1.0f + ep_exp(-x));
+#elif CL_EPI_ACT == 3
+  const float z = fabsf(x) * 0.70710678118654752f;
+  const float t = fast_rcp(__builtin_fmaf(z, 0.4f, 1.0f));
+  float q = 0.05027010291814804f;
+  q = __builtin_fmaf(q, t, -0.18293380737304688f);
+  q = __builtin_fmaf(q, t, 0.16913875937461853f);
+  q = __builtin_fmaf(q, t, -0.005653455853462219f);
+  q = __builtin_fmaf(q, t, 0.14145344495773315f);
+  q = __builtin_fmaf(q, t, 0.1685362011194229f);
+  q = __builtin_fmaf(q, t, 0.20784345269203186f);
+  q = __builtin_fmaf(q, t, 0.22566956281661987f);
+  q = __builtin_fmaf(q, t, 0.22567586600780487f);
+  const float tail = 0.5f * (q * t) * ep_exp(-z * z);       // erfc(|x| / sqrt 2) / 2
+  return x * (x < 0.f ? tail : 1.0f - tail);
+#elif CL_EPI_ACT == 4
+  return x * fast_rcp(1.0f + ep_exp(x * __builtin_fmaf(x * x, -0.07135481282687187f, -1.5957691216057308f)));
+#else
+  return x;
+#endif
+}
+
+// W neighbouring elements from column n of a row on (past the row's end: its last ones again; their results are not stored)
+template <int W> CL_DEVICE void ep_read(const elem_t* row, int n, float (&v)[W]) {
+  if constexpr (W > 1 && CL_N % W == 0) {
+    typedef elem_t piece_t __attribute__((ext_vector_type(W)));
+    const piece_t piece = *reinterpret_cast<const piece_t*>(row + (n < CL_N ? n : CL_N - W));
+#pragma unroll
+    for (int r = 0; r < W; ++r) v[r] = to_f32(piece[r]);
+  } else {
+#pragma unroll
+    for (int r = 0; r < W; ++r) v[r] = to_f32(row[n + r < CL_N ? n + r : CL_N - 1]);
+  }
+}
+// Columns n .. n + W - 1 of row m of the product, in place (n a multiple of W where rows are whole pieces of W)
+template <int W> CL_DEVICE void ep_finish(float (&v)[W], const elem_t* __restrict__ bias, const elem_t* __restrict__ res, int m, int n) {
+  float add[W];
+#if CL_EPI_BIAS
+  ep_read<W>(bias, n, add);
+#pragma unroll
+  for (int r = 0; r < W; ++r) v[r] += add[r];
+#endif
+#pragma unroll
+  for (int r = 0; r < W; ++r) v[r] = ep_act(v[r]);
+#if CL_EPI_RES
+  ep_read<W>(res + (i64)(m < CL_M ? m : CL_M - 1) * CL_N, n, add);
+#pragma unroll
+  for (int r = 0; r < W; ++r) v[r] += add[r];
+#endif
+  (void)add;
+}
+CL_DEVICE f32x4 ep_apply(f32x4 v, const elem_t* __restrict__ bias, const elem_t* __restrict__ res, int m, int n) {
+  float f[4] = {v[0], v[1], v[2], v[3]};
+  ep_finish<4>(f, bias, res, m, n);
+  return (f32x4){f[0], f[1], f[2], f[3]};
+}
+#if CL_EPI_BIAS
+#define EP_BIAS CL_ARG_BIAS
+#else
+#define EP_BIAS nullptr
+#endif
+#if CL_EPI_RES
+#define EP_RES CL_ARG_RES
+#else
+#define EP_RES nullptr
+#endif

@@ -430,9 +430,14 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
 #else
       const float rs = 1.0f;
 #endif
+#if CL_EPI
+      const f32x4 fin = ep_apply(acc[i][j], EP_BIAS, EP_RES, m, n);
+#else
+      const f32x4 fin = acc[i][j] * rs;
+#endif
       elem4 y;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) y[r] = to_elem(acc[i][j][r] * rs);
+      for (int r = 0; r < 4; ++r) y[r] = to_elem(fin[r]);
       st_cols4<CL_N>(CL_ARG_OUT + ((i64)batch * CL_M + m) * CL_N, n, y);
 #endif
     }

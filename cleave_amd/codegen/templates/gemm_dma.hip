@@ -428,7 +428,10 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
     for (int j = 0; j < GD_TN; ++j) {
       const int n = n0 + bn + 16 * j + 4 * g;
       if (n >= CL_N) continue;
-      const f32x4 v = gd_acc_read(acc[i][j]);
+      f32x4 v = gd_acc_read(acc[i][j]);
+#if CL_EPI && CL_SPLITS == 1
+      v = ep_apply(v, EP_BIAS, EP_RES, m, n);
+#endif
 #if CL_SPLITS > 1
       st_cols4<CL_N>(CL_ARG_PACC + (((i64)split * GD_BATCH + batch) * CL_M + m) * CL_N, n, v);
 #else

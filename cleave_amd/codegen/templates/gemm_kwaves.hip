@@ -156,6 +156,9 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
     f32x4 sum = red[q];
 #pragma unroll
     for (int w = 1; w < CL_KW; ++w) sum += red[w * (CL_BM * CL_BN / 4) + q];
+#if CL_EPI
+    sum = ep_apply(sum, EP_BIAS, EP_RES, m, n);
+#endif
     elem4 y;
 #pragma unroll
     for (int r = 0; r < 4; ++r) y[r] = to_elem(sum[r]);

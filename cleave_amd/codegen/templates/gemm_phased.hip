@@ -371,9 +371,14 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
             elem4 e;
+#if CL_EPI
+            const f32x4 fin = ep_apply(acc[h][i][v][j + q], EP_BIAS, EP_RES, m, n0 + GP_HN * v + ecol + 16 * (j + q) + 4 * eg);
+#endif
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-#if CL_SWIGLU
+#if CL_EPI
+              e[r] = to_elem(fin[r]);
+#elif CL_SWIGLU
               const float gate = acc[h][i][1][j + q][r];
               e[r] = to_elem(acc[h][i][0][j + q][r] * gate / (1.0f + __expf(-gate)));
 #else

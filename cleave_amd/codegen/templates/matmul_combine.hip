@@ -85,6 +85,9 @@ CL_COMBINE_NAME(CL_COMBINE_PARAMS) {
     for (int r = 0; r < CL_COMBINE_COLS; ++r) a[r] += d * to_f32(CL_CARG_LB[(i64)rr * CL_N + n + r]);
   }
 #endif
+#if CL_EPI
+  ep_finish<CL_COMBINE_COLS>(a, EP_BIAS, EP_RES, (int)row, n);
+#endif
 #if CL_COMBINE_COLS == 1
   CL_CARG_OUT[row * CL_N + n] = to_elem(a[0] * rs);
 #else

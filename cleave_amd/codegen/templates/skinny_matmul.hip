@@ -366,8 +366,18 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
       const float rs = 1.0f;
 #endif
       elem8 y;
+#if CL_EPI
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const f32x4 fin = ep_apply((f32x4){acc[mt][4 * h][r], acc[mt][4 * h + 1][r], acc[mt][4 * h + 2][r], acc[mt][4 * h + 3][r]},
+                                   EP_BIAS, EP_RES, m, n_base + 8 * c + 4 * h);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[4 * h + j] = to_elem(fin[j]);
+      }
+#else
 #pragma unroll
       for (int j = 0; j < 8; ++j) y[j] = to_elem(acc[mt][j][r] * rs);
+#endif
       if (col_live) st16(CL_ARG_OUT + (i64)m * CL_N + n_base + 8 * c, as_u32x4(y));
 #endif
     }

@@ -6,6 +6,7 @@ the numpy oracle finishes in well under a second.
 
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -53,6 +54,34 @@ def rmsnorm_matmul_eps(x: cl.Tensor["M", "K"], w: cl.Tensor["K", "N"]):
 def swiglu(x: cl.Tensor["M", "K"], w_up: cl.Tensor["K", "N"], w_gate: cl.Tensor["K", "N"]):
     """``(x @ w_up) * silu(x @ w_gate)`` (the reference's ``demo/swiglu.py`` / ``tests/_graphs.py:403-436``)."""
     return (x @ w_up) * cl.silu(x @ w_gate)
+
+
+@functools.lru_cache(maxsize=None)
+def linear_op(act=None, residual=False, bias=True, transposed=False):
+    """``act(x @ w + bias) + residual`` as a ``@jit`` program: a projection with what follows the product in its epilogue.
+    ``act``: None, ``"relu"``, ``"silu"``, ``"gelu"`` or ``"gelu_tanh"``; ``transposed``: the weight is given (N, K)."""
+    follow = {None: lambda y: y, "relu": cl.relu, "silu": cl.silu, "gelu": cl.gelu, "gelu_tanh": lambda y: cl.gelu(y, approximate="tanh")}[act]
+
+    def product(x, w):
+        return x @ (w.mT if transposed else w)
+
+    if bias and residual:
+        def op(x, w, b, r):
+            return follow(product(x, w) + b) + r
+    elif bias:
+        def op(x, w, b):
+            return follow(product(x, w) + b)
+    elif residual:
+        def op(x, w, r):
+            return follow(product(x, w)) + r
+    else:
+        def op(x, w):
+            return follow(product(x, w))
+    op.__annotations__ = {"x": cl.Tensor["M", "K"], "w": cl.Tensor["N", "K"] if transposed else cl.Tensor["K", "N"],
+                          **({"b": cl.Tensor[1, "N"]} if bias else {}), **({"r": cl.Tensor["M", "N"]} if residual else {})}
+    name = "_".join(["linear", *([act] if act else []), *(["bias"] if bias else []), *(["residual"] if residual else []),
+                     *(["nt"] if transposed else [])])
+    return cleave_amd.jit(name=name)(op)
 
 
 @cleave_amd.jit

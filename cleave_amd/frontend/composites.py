@@ -19,6 +19,9 @@ _DUAL = {
     "exp": (lambda x: x.exp(), lambda torch, x: torch.exp(x)),
     "sqrt": (lambda x: x.sqrt(), lambda torch, x: torch.sqrt(x)),
     "silu": (lambda x: x.silu(), lambda torch, x: torch.nn.functional.silu(x)),
+    "relu": (lambda x: x.relu(), lambda torch, x: torch.relu(x)),
+    "gelu": (lambda x, approximate: x.gelu(approximate),
+             lambda torch, x, approximate: torch.nn.functional.gelu(x, approximate=approximate)),
     "max": (lambda x, dim, keepdim: x.max(dim, keepdim=keepdim),
             lambda torch, x, dim, keepdim: x.amax(dim, keepdim=keepdim)),       # values only, no indices
     "matmul": (lambda a, b: a @ b, lambda torch, a, b: grouped_matmul(a, b)),
@@ -44,6 +47,16 @@ def sqrt(x):
 
 def silu(x):
     return _dual("silu", x)
+
+
+def relu(x):
+    return _dual("relu", x)
+
+
+def gelu(x, approximate: str = "none"):
+    """``x * P(N(0, 1) <= x)``; with ``approximate="tanh"`` the usual closed form ``x / 2 * (1 +
+    tanh(sqrt(2 / pi) (x + 0.044715 x^3)))``."""
+    return _dual("gelu", x, approximate)
 
 
 def rsqrt(x):

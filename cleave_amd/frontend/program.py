@@ -122,13 +122,16 @@ VOCABULARY = {
     "exp": _unary(lambda torch: torch.exp),
     "sqrt": _unary(lambda torch: torch.sqrt),
     "silu": _unary(lambda torch: torch.nn.functional.silu),
+    "relu": _unary(lambda torch: torch.relu),
+    "gelu": _unary(lambda torch: torch.nn.functional.gelu),
+    "gelu_tanh": _unary(lambda torch: lambda x: torch.nn.functional.gelu(x, approximate="tanh")),
     "reduce_sum": _reduction("sum"),
     "reduce_max": _reduction("amax"),
     "matmul": OpRule(2, _product,
                      lambda torch, xs, attrs: grouped_matmul(xs[0], xs[1], attrs["trans_A"], attrs["trans_B"]),
                      extras=lambda op: {"trans_A": bool(op.attr("trans_A")), "trans_B": bool(op.attr("trans_B"))}),
 }
-UNARY_KINDS = ("exp", "sqrt", "silu")
+UNARY_KINDS = ("exp", "sqrt", "silu", "relu", "gelu", "gelu_tanh")
 BINARY_KINDS = ("add", "sub", "mul", "div")
 REDUCE_KINDS = ("reduce_sum", "reduce_max")
 

@@ -321,6 +321,11 @@ class Tensor:
     def rsqrt(self):
         return 1.0 / self.sqrt()
 
+    def gelu(self, approximate: str = "none"):
+        if approximate not in ("none", "tanh"):
+            raise SpecError(f"gelu(approximate={approximate!r}): expected 'none' or 'tanh'")
+        return self.program.apply("gelu_tanh" if approximate == "tanh" else "gelu", (self,))
+
     def _reduce(self, kind, dim, keepdim):
         if not keepdim:
             raise SpecError("tile-IR reductions keep the reduced axis; pass keepdim=True")
@@ -347,7 +352,7 @@ def _install_operators():
                                      ("div", "__truediv__", "__rtruediv__")):
         setattr(Tensor, forward, binary(kind, False))
         setattr(Tensor, reflected, binary(kind, True))
-    for kind in ("exp", "sqrt", "silu"):
+    for kind in ("exp", "sqrt", "silu", "relu"):
         setattr(Tensor, kind, (lambda k: lambda self: self.program.apply(k, (self,)))(kind))
 
 

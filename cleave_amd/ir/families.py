@@ -4,7 +4,8 @@ The reference schedules any graph over its op vocabulary by generic tile propaga
 (``python/cleave/schedule/tiling.py:593-882``).  This back end instead recognises whole
 operators and hands each to a hand-written template, so the job here is pattern matching:
 
-    matmul           [batched, grouped-broadcast]  A @ B with optional transposes
+    matmul           [batched, grouped-broadcast]  A @ B with optional transposes; a 2-D product also with
+                     what follows it in its epilogue, act(A @ B + bias) + residual
     rmsnorm_matmul   (x * rsqrt(mean(x^2)[+eps]) [* gamma]) @ w, in either the traced order or
                      the reordered (x [* gamma] @ w) * rsqrt(...) form the superoptimizer emits
                      (tests/integration/graph_structures/rmsnorm_matmul/*valid_1.graph)
@@ -196,6 +197,68 @@ def _try_matmul(view, out):
         return None
     prob = _matmul_problem(a, b, mm.attrs["trans_A"], mm.attrs["trans_B"])
     return "matmul", prob, {"A": a, "B": b}
+
+
+ACTIVATIONS = ("relu", "silu", "gelu", "gelu_tanh")
+
+
+def _addends(view, n, shape):
+    """Peels tensor additions off ``n``: ``(core, row, full)`` with ``n = core + row + full``, where ``row`` (1, N) and ``full``
+    (M, N) are graph inputs or None.  Of a product of one row, where the two look alike, the outer one is ``full``."""
+    row = full = None
+    while _is(n, "add") and n.scalar is None and len(n.inputs) == 2:
+        a, b = view.ins(n)
+        for core, t in ((a, b), (b, a)):
+            if isinstance(core, PlaceHolderNode) or not isinstance(t, PlaceHolderNode):
+                continue
+            if tuple(t.shape) == shape and full is None:
+                full, n = t, core
+                break
+            if tuple(t.shape) == (1, shape[-1]) and row is None:
+                row, n = t, core
+                break
+        else:
+            return n, row, full
+    return n, row, full
+
+
+def _try_linear(view, out):
+    """``act(x @ w + bias) + residual`` over 2-D operands, each part optional (at least one there): the matmul family with an
+    ``epilogue``; operands BIAS (1, N) and RES (M, N).  ``x`` itself may be the residual."""
+    n = view.skip(out)
+    shape = view.shape(n)
+    if shape is None or len(shape) != 2:
+        return None
+    core, row, full = _addends(view, n, shape)
+    act = None
+    if isinstance(core, ComputeOpNode) and core.op in ACTIVATIONS:
+        if row is not None:                        # (act(..) + a row: no kernel adds a row behind the activation)
+            if full is not None or shape[0] != 1:
+                raise LoweringRejected("a row that is added behind the activation has no place in the product's epilogue")
+            row, full = None, row
+        act, inner = core.op, view.ins(core)[0]
+        core, row, early = _addends(view, inner, shape)
+        if early is not None:
+            if shape[0] != 1 or row is not None:
+                raise LoweringRejected("a residual that is added ahead of the activation has no place in the product's epilogue")
+            row = early
+    if not _is(core, "matmul") or (act is None and row is None and full is None):
+        return None
+    a, b = view.ins(core)
+    if not (isinstance(a, PlaceHolderNode) and isinstance(b, PlaceHolderNode)):
+        return None
+    prob = _matmul_problem(a, b, core.attrs["trans_A"], core.attrs["trans_B"])
+    if a is b:
+        raise LoweringRejected("a product of an input with itself is not built")
+    prob["epilogue"] = {"act": act or "none", "bias": row is not None, "res": full is not None}
+    for t in (row, full):
+        if t is not None and t.dtype != a.dtype:
+            raise LoweringRejected(f"bias and residual are in the product's element type, {a.dtype}, got {t.dtype}")
+    if row is not None and any(row is t for t in (a, b, full)):
+        raise LoweringRejected("the bias is an input of its own")
+    if full is not None and full is b:
+        raise LoweringRejected("the weight cannot be the residual as well")
+    return "matmul", prob, {"A": a, "B": b, **({"BIAS": row} if row is not None else {}), **({"RES": full} if full is not None else {})}
 
 
 def _try_swiglu(view, out):
@@ -509,7 +572,7 @@ def _try_attention(view, out):
 
 
 _MATCHERS = (_try_rmsnorm_matmul, _try_swiglu, _try_lora, _try_matmul_rowsum, _try_rowsum, _try_attention,
-             _try_chained_matmul, _try_matmul)
+             _try_chained_matmul, _try_linear, _try_matmul)
 
 
 def recognize(graph: Graph) -> Lowered:

@@ -42,7 +42,7 @@ class PlaceHolderNode(Node):
 
 @dataclass(eq=False)
 class ComputeOpNode(Node):
-    op: str = ""                      # matmul add sub mul div exp sqrt silu reduce_sum reduce_max split
+    op: str = ""                      # matmul add sub mul div exp sqrt silu relu gelu gelu_tanh reduce_sum reduce_max split
     inputs: list = field(default_factory=list)   # Node operands, in order
     scalar: float | None = None       # the constant operand of a scalar binary
     scalar_on_left: bool = False
@@ -152,7 +152,7 @@ def to_ir(structure, symbol_map=None, dtype: str = "float16", out_dtype: str | N
     return Graph(nodes, dtype, name)
 
 
-_POINTWISE = ("add", "sub", "mul", "div", "exp", "sqrt", "rsqrt", "silu")
+_POINTWISE = ("add", "sub", "mul", "div", "exp", "sqrt", "rsqrt", "silu", "relu", "gelu", "gelu_tanh")
 
 
 def _split_shape(shape, dim, factor) -> tuple:

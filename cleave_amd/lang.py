@@ -14,7 +14,7 @@ from .frontend import tensor as _tensor
 
 _EAGER = {
     _tensor: "DType Dim Scalar Split Tensor bf16 dims f16 f32 i32",
-    _ops: "exp matmul max mean rms_norm rsqrt silu sqrt sum",
+    _ops: "exp gelu matmul max mean relu rms_norm rsqrt silu sqrt sum",
     _paged: "PageTable ScheduleHints paged_gather softmax",
 }
 _LATE = {"Tolerance": (".runtime.validate", "Tolerance"), "workloads": (".frontend.paged", "workloads")}

@@ -93,6 +93,8 @@ def split_stages(graph: StageGraph, factor: int) -> list:
     if low.family == "lora":
         # the rank update happens in the combine, which therefore also reads the up factor
         comb_ins.append(low.operands["LB"])
+    # (what follows a product follows its sum: bias and residual are the combine's to read)
+    comb_ins += [low.operands[r] for r in ("BIAS", "RES") if r in low.operands]
     partial = StageGraph(graph, low, "partial", factor, outputs=part_outs)
     combine = StageGraph(graph, low, "combine", factor, placeholders=comb_ins)
     partial.name, combine.name = f"{graph.name}.partial", f"{graph.name}.combine"

@@ -96,6 +96,21 @@ def _mm_operands(low, feed):
     return a, b  # (batch, M, K), (batch, K, N)
 
 
+def _epilogue(low, feed, y):
+    """What follows a product before it is rounded: ``act(y + bias) + residual``."""
+    import torch
+
+    ep = low.problem.get("epilogue")
+    if not ep:
+        return y
+    if ep["bias"]:
+        y = y + feed[low.operands["BIAS"].name].float()
+    gelu = torch.nn.functional.gelu
+    y = {"none": lambda t: t, "relu": torch.relu, "silu": torch.nn.functional.silu, "gelu": gelu,
+         "gelu_tanh": lambda t: gelu(t, approximate="tanh")}[ep["act"]](y)
+    return y + feed[low.operands["RES"].name].float() if ep["res"] else y
+
+
 def _eval_matmul(low, feed, role, factor, out_dtype):
     import torch
 
@@ -117,7 +132,7 @@ def _eval_matmul(low, feed, role, factor, out_dtype):
     y = a @ b
     if norm:
         y = y * torch.rsqrt((raw ** 2).mean(-1, keepdim=True) + p["eps"])
-    return [y.to(out_dtype)]
+    return [_epilogue(low, feed, y).to(out_dtype)]
 
 
 def _eval_swiglu(low, feed, out_dtype):
@@ -139,7 +154,7 @@ def _eval_matmul_combine(low, feed, out_dtype, out_shape):
     if low.family == "rmsnorm_matmul":
         ss = feed["PlaceHolder_PSS"].float().sum(0)
         acc = acc * torch.rsqrt(ss / p["K"] + p["eps"]).unsqueeze(-1)
-    return [acc.to(out_dtype).reshape(out_shape)]
+    return [_epilogue(low, feed, acc.reshape(out_shape)).to(out_dtype)]
 
 
 def _attn_scores(low, feed):

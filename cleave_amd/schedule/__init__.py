@@ -154,11 +154,15 @@ def apply_tiling(cand: TileDict) -> KernelPlan:
         for ph in graph.placeholders:
             params.append(ParamSpec(ph.name, ph.dtype, tuple(ph.shape), "input"))
             operands[by_node[id(ph)]] = ph.name
+            if low.operands.get("RES") is ph:              # (x itself may be the residual of its product)
+                operands.update({r: ph.name for r, n in low.operands.items() if n is ph})
     else:
         keep_role = {id(n): r for r, n in low.operands.items()}      # an original input a combine reads (LoRA's up factor)
         for ph in graph.placeholders:
             params.append(ParamSpec(ph.name, ph.dtype, tuple(ph.shape), "input"))
             operands[keep_role.get(id(ph), ph.name.replace("PlaceHolder_", ""))] = ph.name
+            if low.operands.get("RES") is ph:
+                operands["RES"] = ph.name
     if role == "partial":
         for out, (bname, shape, dt) in zip(graph.outputs, partial_buffers(low, cand.split_factor)):
             params.append(ParamSpec(out.name, dt, tuple(shape), "output"))
