@@ -561,6 +561,11 @@ class HipCodeGen:
                 raise CodegenError("SKEW (split ranges skewed between even and odd XCDs, in thousandths of a pair's steps, "
                                    "1..500) needs an even split count, a grid of whole groups of eight unit tiles and no chunked items")
             unit.define("CL_SKEW", skew)
+        if p.get("window"):
+            if chunk_pages:
+                raise CodegenError("a window has no chunked items")
+            unit.define("CL_WINDOW", p["window"])
+            unit.define("CL_SINKS", p["sinks"])
         unit.define("CL_PAGED", paged)
         unit.define("CL_PAGE_SIZE", p.get("page_size", 1))
         unit.define("CL_KV_HEADS", p.get("kv_heads", 1))
@@ -681,7 +686,7 @@ class HipCodeGen:
         if d % 32 or not (d % 128 == 0 or d == 64) or 16 % group or p["kv_heads"] > 16:
             raise CodegenError("prefill needs head_dim 64 or k*128, a head group dividing 16 and at most 16 kv heads")
         for k, v in (("CL_HEAD_DIM", d), ("CL_KV_HEADS", p["kv_heads"]), ("CL_Q_HEADS", p["q_heads"]),
-                     ("CL_RAGGED", bool(p["ragged"]))):
+                     ("CL_RAGGED", bool(p["ragged"])), *((("CL_WINDOW", p["window"]), ("CL_SINKS", p["sinks"])) if p.get("window") else ())):
             unit.define(k, v)
         for role, macro in (("Q", "CL_ARG_Q"), ("K", "CL_ARG_K"), ("V", "CL_ARG_V"), ("QINDPTR", "CL_ARG_QINDPTR"),
                             ("INDPTR", "CL_ARG_INDPTR"), ("INDICES", "CL_ARG_INDICES")):

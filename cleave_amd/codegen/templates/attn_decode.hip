@@ -37,7 +37,17 @@
 //                per kv head, so that the eight waves together stream whole contiguous token
 //                rows of the cache and a long request costs many items rather than long ones.
 
+//   CL_WINDOW, CL_SINKS  paged only: the query sees the request's last CL_WINDOW keys and its first CL_SINKS ones.  Steps are
+//                numbered without the ones in between (step s is 32-token step s of the request up to the sinks' last one and
+//                s + skip behind it), so that splits share out what is seen; the ragged edges are masked.
+
 #define ATT_RAISE_BY 8.0f
+#ifndef CL_WINDOW
+#define CL_WINDOW 0
+#endif
+#if CL_WINDOW && !CL_PAGED
+#error "a window: paged keys"
+#endif
 #ifndef CL_CHUNK_PAGES
 #define CL_CHUNK_PAGES 0
 #endif
@@ -59,6 +69,17 @@
 #error "skewed split ranges: an even number of splits, no chunked items"
 #endif
 #define ATT_STEP 32
+#if CL_WINDOW
+#define ATT_SINK_STEPS ((CL_SINKS + ATT_STEP - 1) / ATT_STEP)
+#define ATT_T0(u, s) (((s) < ATT_SINK_STEPS ? (s) : (s) + (u).skip) * ATT_STEP)
+#define ATT_SEES(u, t) ((t) < (u).kv_len && ((t) >= (u).kv_len - CL_WINDOW || (t) < CL_SINKS))
+// (a key that is not seen is not read either: its page may be another's by now, and weight 0 times an infinite value is not 0)
+#define ATT_READ(u, t, last) (ATT_SEES(u, t) ? (t) : (last))
+#else
+#define ATT_READ(u, t, last) ((t) < (last) ? (t) : (last))
+#define ATT_T0(u, s) ((s) * ATT_STEP)
+#define ATT_SEES(u, t) ((t) < (u).kv_len)
+#endif
 #define ATT_KJ (CL_HEAD_DIM / 32)            // score MFMAs per 16 tokens
 #define ATT_VC ((CL_VDIM + 127) / 128)       // 128-wide value chunks
 #define ATT_ROW_TILES ((CL_ROWS + 15) / 16)
@@ -69,6 +90,9 @@ struct AttUnit {
   const elem_t* v;
   i64 k_stride, v_stride;   // elements between consecutive tokens of K and of V (their widths may differ)
   int kv_len;           // valid tokens
+#if CL_WINDOW
+  int skip;             // 32-token steps between the sinks' last one and the window's first one
+#endif
   int rows;             // real rows in this tile (1..16)
   const int* pages;     // paged: this request's slice of the page table
   int page_reg;         // chunked items: lane i holds the (clamped) id of the slice's page i
@@ -139,7 +163,7 @@ CL_DEVICE void att_load(const AttUnit& u, int t0, int c, int g, AttTile& tile) {
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     int t = t0 + 16 * h + c;
-    t = t < last ? t : last;
+    t = ATT_READ(u, t, last);
     const elem_t* row = u.k + att_token_row(u, t) * u.k_stride + 8 * g;
 #pragma unroll
     for (int j = 0; j < ATT_KJ; ++j) tile.k[h][j] = ld16(row + 32 * j);
@@ -147,7 +171,7 @@ CL_DEVICE void att_load(const AttUnit& u, int t0, int c, int g, AttTile& tile) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     int t = t0 + (e < 4 ? 4 * g + e : 16 + 4 * g + (e - 4));
-    t = t < last ? t : last;
+    t = ATT_READ(u, t, last);
     const elem_t* row = u.v + att_token_row(u, t) * u.v_stride;
 #pragma unroll
     for (int vc = 0; vc < ATT_VC; ++vc) {
@@ -293,7 +317,13 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
 #endif
 
   // This split's steps: ceil(n_steps / SPLITS) each; a trailing split may own none.
+#if CL_WINDOW
+  u.skip = (u.kv_len > CL_WINDOW ? u.kv_len - CL_WINDOW : 0) / ATT_STEP - ATT_SINK_STEPS;
+  u.skip = u.skip > 0 ? u.skip : 0;
+  const int n_steps = (u.kv_len + ATT_STEP - 1) / ATT_STEP - u.skip;
+#else
   const int n_steps = (u.kv_len + ATT_STEP - 1) / ATT_STEP;
+#endif
 #if CL_CHUNK_PAGES
   const int step_begin = 0, step_end = n_steps;      // the item is the unit of work: no further cut
   (void)split;
@@ -379,9 +409,9 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
 #define ATT_ONE_STEP(R, STEP, LOAD)                                                                 \
     {                                                                                               \
       ATT_LOCKSTEP()                                                                                \
-      if (LOAD) att_load(u, ((STEP) + CL_PREFETCH * ATT_WSTRIDE) * ATT_STEP, c, g, ring[((R) + CL_PREFETCH) % (CL_PREFETCH + 1)]); \
+      if (LOAD) att_load(u, ATT_T0(u, (STEP) + CL_PREFETCH * ATT_WSTRIDE), c, g, ring[((R) + CL_PREFETCH) % (CL_PREFETCH + 1)]); \
       const AttTile& cur = ring[R];                                                                 \
-      const int t0 = (STEP) * ATT_STEP;                                                             \
+      const int t0 = ATT_T0(u, STEP);                                                               \
                                                                                                     \
       float s[8];                                                                                   \
 _Pragma("unroll")                                                                                   \
@@ -392,7 +422,7 @@ _Pragma("unroll")                                                               
 _Pragma("unroll")                                                                                   \
         for (int q = 0; q < 4; ++q) {                                                               \
           const int t = t0 + 16 * h + 4 * g + q;                                                    \
-          s[4 * h + q] = t < u.kv_len ? st[q] * scale2 : CL_NEG_BIG;                                \
+          s[4 * h + q] = ATT_SEES(u, t) ? st[q] * scale2 : CL_NEG_BIG;                              \
         }                                                                                           \
       }                                                                                             \
       float mx = s[0];                                                                              \
@@ -437,7 +467,7 @@ _Pragma("unroll")                                                               
   if (step0 < step_end) {
 #pragma unroll
     for (int i = 0; i < CL_PREFETCH; ++i)
-      if (step0 + i * ATT_WSTRIDE < step_end) att_load(u, (step0 + i * ATT_WSTRIDE) * ATT_STEP, c, g, ring[i]);
+      if (step0 + i * ATT_WSTRIDE < step_end) att_load(u, ATT_T0(u, step0 + i * ATT_WSTRIDE), c, g, ring[i]);
     int base = step0;
     for (; base + 2 * CL_PREFETCH * ATT_WSTRIDE < step_end; base += (CL_PREFETCH + 1) * ATT_WSTRIDE) {
 #pragma unroll

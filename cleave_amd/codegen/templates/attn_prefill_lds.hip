@@ -59,6 +59,10 @@
 //
 // CL_PF_XCD / CL_PF_REVERSE (default 1) switch the XCD mapping and the walking order.
 //
+// CL_WINDOW, CL_SINKS (paged modes): a row sees the last CL_WINDOW keys up to its own and the request's first CL_SINKS ones.
+// Steps are numbered without the ones that no row of the item sees: step s is 32-key tile s of the request up to the sinks' last
+// tile and tile s + skip behind it; tiles that a row of the wave sees in part are masked at either end.
+//
 //   CL_HEAD_DIM (multiple of 64)  CL_KV_HEADS  CL_Q_HEADS (group divides 16)  CL_RAGGED
 //   run-time: batch, total_q, n_idx (table length / total_kv), num_pages (table form), sm_scale
 
@@ -85,6 +89,13 @@
 #endif
 #ifndef CL_KNORM
 #define CL_KNORM 0
+#endif
+#ifndef CL_WINDOW
+#define CL_WINDOW 0
+#define CL_SINKS 0
+#endif
+#if CL_WINDOW && CL_DENSE
+#error "a window: ragged queries"
 #endif
 #if CL_DENSE && !CL_RAGGED
 #error "dense operands have consecutive key rows (CL_RAGGED)"
@@ -246,7 +257,17 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
   const char* kbase = reinterpret_cast<const char*>(CL_ARG_K) + (i64)head * CL_HEAD_DIM * 2;
   const char* vbase = reinterpret_cast<const char*>(CL_ARG_V) + (i64)head * CL_VDIM * 2;
 #endif
-  const int n_steps = (ext + PL_STEP - 1) / PL_STEP;
+#if CL_WINDOW
+  // (the item's first row begins its window first)
+  constexpr int sink_steps = (CL_SINKS + PL_STEP - 1) / PL_STEP;
+  const int first_key = off + (lo - q0) - CL_WINDOW + 1;
+  int skip = (first_key > 0 ? first_key : 0) / PL_STEP - sink_steps;
+  skip = skip > 0 ? skip : 0;
+#else
+  constexpr int sink_steps = 0, skip = 0;
+#endif
+  auto tile_of = [&](int s) __attribute__((always_inline)) { return CL_WINDOW && s >= sink_steps ? s + skip : s; };
+  const int n_steps = (ext + PL_STEP - 1) / PL_STEP - skip;
   const unsigned tiles_byte = (unsigned)(size_t)(__attribute__((address_space(3))) elem_t*)pl_tiles;
 
   // Loads of one step, this wave's share: key rows 8 wave + lane / 8 of every 64-feature panel, the chunk for slot
@@ -254,7 +275,7 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
   // same number of loads at every wait; positions past the item's last key repeat it.
   const int my_r = 8 * wave + (lane >> 3);
   const int chunk_byte = 16 * ((lane & 7) ^ pl_swz(my_r));
-  const int last_step = n_steps - 1, tail_r = ext - 1 - PL_STEP * last_step;      // last row of the last step
+  const int last_step = n_steps - 1, tail_r = ext - 1 - PL_STEP * (last_step + skip);      // last row of the last step
   const int row_tail = my_r < tail_r ? my_r : tail_r;
 #if CL_RAGGED
   // consecutive rows: a scalar base per step and one of two lane offsets (whole step / last step)
@@ -273,7 +294,7 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
       pl_dma16<0>(kbase + ((i64)feat * CL_SKV + s * PL_STEP) * 2 + 16 * piece, dst + (unsigned)(P * PL_PANEL * 2));
     });
 #elif CL_RAGGED
-    const char* base = kbase + (i64)(kv0 + s * PL_STEP) * krow_bytes;
+    const char* base = kbase + (i64)(kv0 + tile_of(s) * PL_STEP) * krow_bytes;
     const unsigned off = s == last_step ? koff[1] : koff[0];
     pl_static_for<decltype(lo_c)::value, decltype(hi_c)::value>([&](auto p) __attribute__((always_inline)) {
       constexpr int P = decltype(p)::value;
@@ -292,7 +313,7 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
     s = s < last_step ? s : last_step;
     const unsigned dst = tiles_byte + (unsigned)((PL_STAGES * PL_KIMG + slot * PL_VIMG) * 2 + wave * 1024);
 #if CL_RAGGED
-    const char* base = vbase + (i64)(kv0 + s * PL_STEP) * vrow_bytes;
+    const char* base = vbase + (i64)(kv0 + tile_of(s) * PL_STEP) * vrow_bytes;
     const unsigned off = s == last_step ? voff[1] : voff[0];
     pl_static_for<decltype(lo_c)::value, decltype(hi_c)::value>([&](auto p) __attribute__((always_inline)) {
       constexpr int P = decltype(p)::value;
@@ -309,7 +330,7 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
   };
 #if !CL_RAGGED
   auto key_pos = [&](int s) __attribute__((always_inline)) {
-    return PL_STEP * (s < last_step ? s : last_step) + (s < last_step ? my_r : row_tail);
+    return PL_STEP * tile_of(s < last_step ? s : last_step) + (s < last_step ? my_r : row_tail);
   };
   auto row_of = [&](int s) __attribute__((always_inline)) { return pl_clamp(CL_ARG_INDICES[kv0 + key_pos(s)], 0, num_pages - 1); };
   // In the loop the lane's table entry travels like the tiles do, global -> LDS on the kernel's
@@ -406,10 +427,23 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
   int n_full = n_steps;
   if (32 * wave < n_rows) {
     const int first_limit = row_limit(32 * wave);
-    n_full = first_limit < 0 ? 0 : (first_limit + 1) / PL_STEP;
+    n_full = first_limit < 0 ? 0 : (first_limit + 1) / PL_STEP - skip;
     n_full = n_full < n_steps ? n_full : n_steps;
   }
   n_full = __builtin_amdgcn_readfirstlane(n_full);
+#if CL_WINDOW
+  // ... and whose window every row has begun before them: the wave's last row begins its own last.  (Of the sinks' tiles before
+  // that all are masked: one of a hundred steps.)
+  int n_low = 0;
+  if (32 * wave < n_rows) {
+    const int last_row = 32 * wave + 31 < n_rows ? 32 * wave + 31 : n_rows - 1;
+    const int begun = row_limit(last_row) - CL_WINDOW + 1;
+    n_low = begun > 0 ? (begun + PL_STEP - 1) / PL_STEP - skip : 0;
+  }
+  n_low = __builtin_amdgcn_readfirstlane(n_low);
+#else
+  constexpr int n_low = 0;
+#endif
 
   // key fragment of 16-key half h and 32-feature block j out of the K image in stage SLOT: a 16-byte read, which feeds the
   // wave's two row tiles
@@ -502,9 +536,18 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
   auto mask = [&](f32x4 (&sc)[2][2], int step) __attribute__((always_inline)) {
 #pragma unroll
     for (int rt = 0; rt < 2; ++rt) {
-      const int room = lim_rel[rt] - step * PL_STEP;
+      const int room = lim_rel[rt] - tile_of(step) * PL_STEP;
+#if CL_WINDOW
+      const int sink_room = CL_SINKS - 4 * g - tile_of(step) * PL_STEP;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int at = 16 * (i >> 2) + (i & 3);
+        sc[rt][i >> 2][i & 3] = at <= room && (at > room - CL_WINDOW || at < sink_room) ? sc[rt][i >> 2][i & 3] : CL_NEG_INF;
+      }
+#else
 #pragma unroll
       for (int i = 0; i < 8; ++i) sc[rt][i >> 2][i & 3] = 16 * (i >> 2) + (i & 3) <= room ? sc[rt][i >> 2][i & 3] : (CL_LINEAR ? 0.f : CL_NEG_INF);
+#endif
     }
   };
   // the largest of this lane's eight scores of a row (in the compiler's sight: it keeps the wait states between a matrix op
@@ -528,7 +571,7 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
   read_keys(PlC<1>{}, 0);
 #if !CL_LINEAR && CL_HEAD_DIM <= 192
   // (the first reference points, so that the first weights need not be taken twice; the widest heads have no registers for it)
-  if (n_full == 0) mask(st, 0);
+  if (n_full <= 0 || n_low > 0) mask(st, 0);
 #pragma unroll
   for (int rt = 0; rt < 2; ++rt) {
     const float mx = pl_max_over_groups(step_max(st[rt])) * scale2;
@@ -563,7 +606,7 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
       issue_k(step + 4, (S + 4) % PL_STAGES, PlC<LO - VL>{}, PlC<HI - VH>{}, row_k);
     };
     __builtin_amdgcn_sched_barrier(0);
-    if (step >= n_full) mask(st, step);
+    if (step >= n_full || step < n_low) mask(st, step);
     __builtin_amdgcn_sched_barrier(0);
 
     elem8 pf[2];

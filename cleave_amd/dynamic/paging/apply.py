@@ -158,8 +158,15 @@ def _check_tiling(spec, dense, split: bool = False) -> None:
     if dense.query_rows < spec.group:
         raise UnsupportedTiling(f"a block's query tile holds {dense.query_rows} rows but the head group needs "
                                 f"{spec.group}; re-tile with at least {spec.group} query rows")
+    if getattr(spec, "shared_input", None) is not None:
+        raise UnsupportedTiling("no kernel reads shared pages yet")
     if dense.head_dim % 32 or not (dense.head_dim % 128 == 0 or dense.head_dim == 64):
         raise UnsupportedTiling(f"head_dim {dense.head_dim} is not 64 or a multiple of 128")
+
+
+def _limits(spec: PagingSpec) -> dict:
+    """What a window adds to a plan's problem."""
+    return {} if spec.window is None else {"window": spec.window, "sinks": spec.sinks}
 
 
 def _paged_params(spec: PagingSpec, dense: DenseAttention):
@@ -194,7 +201,7 @@ def _paged_outputs(spec: PagingSpec, dense: DenseAttention):
 def _paged_problem(spec: PagingSpec, dense: DenseAttention) -> dict:
     return {"paged": True, "page_size": spec.page_size, "kv_heads": spec.num_kv_heads,
             "q_heads": spec.num_qo_heads, "group": spec.group, "sq": 1, "head_dim": dense.head_dim,
-            "vdim": dense.head_dim, "emit_lse": bool(spec.emit_lse), "units": None, "skv": 0, "scale": 1.0,
+            "vdim": dense.head_dim, "emit_lse": bool(spec.emit_lse), "units": None, "skv": 0, "scale": 1.0, **_limits(spec),
             "dim_names": {"batch": spec.batch_dim, "num_pages": spec.pages_dim, "n_idx": spec.index_dim}}
 
 
@@ -249,7 +256,10 @@ def _prefill_plan(spec: PagingSpec, dense: DenseAttention, shared: bool | None =
     tiling entries of the shared kernel (each becomes a ``CL_PF_<name>`` definition)."""
     d, dt = dense.head_dim, dense.dtype
     if shared is None:
-        shared = dense.waves >= 4 and d % 64 == 0
+        shared = spec.window is not None or (dense.waves >= 4 and d % 64 == 0)
+    if spec.window is not None and (not shared or d % 64 or d > 256):
+        raise UnsupportedTiling("a window is built into the kernel whose waves share key tiles, for heads that are a multiple of 64 "
+                                f"and at most 256 wide (head_dim {d})")
     ragged = spec.kind == RAGGED_PREFILL_CAUSAL
     tq = spec.tokens_dim
     ph = lambda n: f"PlaceHolder_{n}"  # noqa: E731
@@ -278,7 +288,7 @@ def _prefill_plan(spec: PagingSpec, dense: DenseAttention, shared: bool | None =
         {"total_q": tq, "num_pages": spec.pages_dim, "n_idx": spec.index_dim}
     problem = {"paged": True, "prefill": True, "ragged": ragged, "kv_heads": spec.num_kv_heads,
                "q_heads": spec.num_qo_heads, "group": spec.group, "head_dim": d, "vdim": d,
-               "emit_lse": bool(spec.emit_lse), "units": None, "skv": 0, "sq": 0, "scale": 1.0, "dim_names": dim_names}
+               "emit_lse": bool(spec.emit_lse), "units": None, "skv": 0, "sq": 0, "scale": 1.0, **_limits(spec), "dim_names": dim_names}
     threads, rows = (256, 128) if shared else (spec.num_kv_heads * 64, 16)
     return KernelPlan(template="attn_prefill", role="main", family="attention", dtype=dense.dtype,
                       extra={"derived_dims": [("batch", f"{spec.indptr_dim} - 1")]}, problem=problem,
@@ -290,6 +300,8 @@ def prefill_variants(plan: KernelPlan, spec) -> list:
     """Both kernels of a causal prefill layer at ``plan``'s dense tiling (the search times each)."""
     dense = read_dense_attention(plan)
     _check_tiling(spec, dense)
+    if spec.window is not None:
+        return [_prefill_plan(spec, dense, shared=True)]
     return [_prefill_plan(spec, dense, shared=s) for s in ((False, True) if dense.head_dim % 64 == 0 else (False,))]
 
 
@@ -457,6 +469,8 @@ def build_split_decode(spec, dense: DenseAttention, split: int, comb: CombineTil
     # split-major partials: one request's splits sit one stride apart
     # (python/cleave/dynamic/paging/tensor_maps.py:41-69)
     if dense.chunk_pages:
+        if spec.window is not None:
+            raise UnsupportedTiling("items of a page table are cut from all of a request's pages: a window has the fixed split")
         if dense.chunk_pages < -1 or dense.chunk_pages > max_chunk_pages(spec) or dense.query_rows > 16 \
                 or spec.num_kv_heads > 16:
             raise UnsupportedTiling(f"chunked items need chunk_pages in 1..{max_chunk_pages(spec)} (or -1), one 16-row "

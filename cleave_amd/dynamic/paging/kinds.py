@@ -31,6 +31,8 @@ _READERS = {
     "last_page_len_input": SLAB_KINDS,
     "query_indptr_input": CAUSAL_KINDS,
     "grid_order": (PAGED_DECODE, PAGED_DECODE_SLAB),
+    "shared_input": (PAGED_DECODE, PAGED_DECODE_SLAB),
+    "shared_dim": (PAGED_DECODE, PAGED_DECODE_SLAB),
 }
 _MLA_READERS = {
     "batch_dim": (MLA_PAGED_DECODE,),

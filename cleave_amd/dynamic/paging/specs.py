@@ -91,6 +91,10 @@ class PagingSpec:
     rasterization: int | None = 1
     warp_policy: str = "cols"
     grid_order: tuple = ("batch", "head")
+    window: int | None = None           # keys a query sees up to its own position (None: all of them) ...
+    sinks: int = 0                      # ... beside the first ones of its request
+    shared_input: str | None = None     # pages every request begins with (decode)
+    shared_dim: str | None = None
 
     @property
     def group(self) -> int:
@@ -98,7 +102,7 @@ class PagingSpec:
         return self.num_qo_heads // self.num_kv_heads
 
     def validate(self) -> None:
-        _whole_numbers(self, ("num_qo_heads", "num_kv_heads", "page_size", "rasterization"))
+        _whole_numbers(self, ("num_qo_heads", "num_kv_heads", "page_size", "rasterization", "window", "sinks"))
         q, kv, page = self.num_qo_heads, self.num_kv_heads, self.page_size
         slab = self.kind in SLAB_KINDS
         _check([
@@ -119,10 +123,18 @@ class PagingSpec:
         ])
         read = FIELDS_READ[self.kind]
         _only_read_fields_are_set(self, OPTIONAL_FIELDS, read)
-        per_layer = [getattr(self, n) for n in ("index_input", "last_page_len_input", "query_indptr_input") if n in read]
+        _check([
+            (self.window is None or 1 <= self.window < 1 << 30, f"window={self.window} leaves a query without its own key"),
+            (0 <= self.sinks < 1 << 30, f"sinks={self.sinks} is no number of keys"),
+            (self.window is not None or self.sinks == 0, f"sinks={self.sinks} without a window changes nothing"),
+            ((self.shared_input is None) == (self.shared_dim is None), "shared pages need an input and its extent's name"),
+            (self.shared_input is None or self.window is None, "shared pages are built without a window"),
+        ])
+        per_layer = [getattr(self, n) for n in ("index_input", "last_page_len_input", "query_indptr_input", "shared_input")
+                     if n in read and getattr(self, n) is not None]
         _distinct("input names", [self.indptr_input, self.query_input, self.scale_input, *self.cache_inputs, *per_layer])
-        extents = [getattr(self, n) for n in ("batch_dim", "tokens_dim", "kv_tokens_dim", "pages_dim", "index_dim")
-                   if n in read]
+        extents = [getattr(self, n) for n in ("batch_dim", "tokens_dim", "kv_tokens_dim", "pages_dim", "index_dim", "shared_dim")
+                   if n in read and getattr(self, n) is not None]
         _distinct("symbolic extent names", [self.indptr_dim, self.scale_input, *extents])
         _check([
             (self.warp_policy in WARP_POLICIES, f"unsupported warp policy {self.warp_policy!r}"),

@@ -101,42 +101,51 @@ def paged_tokens(kv_indices, base, kv_len, page_size):
     return page_of, slot_of
 
 
-def gqa_paged_decode_inputs(dims, kv_lens, page_size=1, scale=None, dtype=None, device="cuda", seed=SEED):
-    """The operator's arguments in declaration order: q, k_cache, v_cache, kv_indptr, kv_indices,
-    [kv_last_page_len], sm_scale.  ``dims`` = (batch, qo_heads, kv_heads, head_dim, num_pages, n_idx)."""
+def gqa_paged_decode_inputs(dims, kv_lens, page_size=1, scale=None, dtype=None, device="cuda", seed=SEED, shared=0):
+    """The operator's arguments in declaration order: q, k_cache, v_cache, [shared_indices,] kv_indptr, kv_indices,
+    [kv_last_page_len], sm_scale.  ``dims`` = (batch, qo_heads, kv_heads, head_dim, num_pages, n_idx); ``shared``: pages
+    that all requests begin with (``kv_lens`` counts the tokens behind them)."""
     torch = _torch()
     dtype = dtype or torch.bfloat16
     batch, hq, hkv, d, num_pages, n_idx = dims[:6]
     gen = _generator(device, seed)
     pages_per_req = [-(-int(n) // page_size) for n in kv_lens]
-    kv_indices = _pad_indices(_page_table(num_pages, sum(pages_per_req), device, seed), n_idx)
+    table = _page_table(num_pages, shared + sum(pages_per_req), device, seed)
+    kv_indices = _pad_indices(table[shared:], n_idx)
 
     def randn(*shape):
         return torch.randn(*shape, device=device, dtype=dtype, generator=gen)
 
     args = [randn(batch, hq, d), randn(num_pages, page_size, hkv, d), randn(num_pages, page_size, hkv, d),
-            _i32(_indptr(pages_per_req), device), kv_indices]
+            *([table[:shared].clone()] if shared else []), _i32(_indptr(pages_per_req), device), kv_indices]
     if page_size != 1:
         args.append(_i32([n - (p - 1) * page_size if p else 0 for n, p in zip(kv_lens, pages_per_req)], device))
     args.append(float(d) ** -0.5 if scale is None else float(scale))
     return args
 
 
-def gqa_paged_decode_reference(dims, kv_lens, page_size=1, dtype=None):
+def gqa_paged_decode_reference(dims, kv_lens, page_size=1, dtype=None, window=None, sinks=0, shared=0):
     torch = _torch()
     dtype = dtype or torch.bfloat16
     batch, hq, hkv, d = dims[:4]
     group = hq // hkv
 
-    def reference(q, k_cache, v_cache, kv_indptr, kv_indices, *rest):
-        sm_scale = rest[-1]
+    def reference(q, k_cache, v_cache, *rest):
+        sm_scale, (kv_indptr, kv_indices) = rest[-1], rest[1:3] if shared else rest[:2]
+        first = paged_tokens(rest[0], 0, shared * page_size, page_size) if shared else None
         out = torch.zeros(batch, hq, d, device=q.device, dtype=dtype)
         lse = torch.full((batch, hq), NEG_INF, device=q.device, dtype=torch.float32)
         starts = kv_indptr.tolist()
         for b, kv_len in enumerate(kv_lens):
-            if kv_len <= 0:
+            if kv_len <= 0 and not shared:
                 continue
             page_of, slot_of = paged_tokens(kv_indices, int(starts[b]), int(kv_len), page_size)
+            if shared:
+                page_of, slot_of = torch.cat([first[0], page_of]), torch.cat([first[1], slot_of])
+            if window is not None:
+                at = torch.arange(int(kv_len), device=q.device)
+                seen = (at >= int(kv_len) - window) | (at < sinks)
+                page_of, slot_of = page_of[seen], slot_of[seen]
             kk = k_cache[page_of, slot_of].repeat_interleave(group, dim=1)
             vv = v_cache[page_of, slot_of].repeat_interleave(group, dim=1)
             o, l = _attend(q[b:b + 1], kk, vv, sm_scale)
@@ -211,13 +220,16 @@ def mla_paged_decode_reference(dims, kv_lens, dtype=None):
 
 
 # ----------------------------------------------------------------------------- causal prefill
-def causal_keep(q_len, kv_len, device):
+def causal_keep(q_len, kv_len, device, window=None, sinks=0):
     """End-aligned causal mask (``python/cleave/dynamic/reference.py:129-133``): keep
-    ``kv_pos <= kv_len - q_len + q_pos``; (q_len, kv_len) bool."""
+    ``kv_pos <= kv_len - q_len + q_pos``; (q_len, kv_len) bool.  With a ``window``, of those the
+    last ``window`` and the request's first ``sinks``."""
     torch = _torch()
     q_pos = torch.arange(q_len, device=device)[:, None]
     kv_pos = torch.arange(kv_len, device=device)[None, :]
-    return kv_pos <= (kv_len - q_len) + q_pos
+    own = (kv_len - q_len) + q_pos
+    keep = kv_pos <= own
+    return keep if window is None else keep & ((kv_pos > own - window) | (kv_pos < sinks))
 
 
 def gqa_paged_prefill_inputs(dims, q_lens, kv_lens, scale=None, dtype=None, device="cuda", seed=SEED):
@@ -254,7 +266,7 @@ def gqa_ragged_prefill_inputs(dims, q_lens, kv_lens, scale=None, dtype=None, dev
             _i32(_indptr(kv_lens), device), float(d) ** -0.5 if scale is None else float(scale)]
 
 
-def _prefill_reference(hq, hkv, d, total_q, q_lens, kv_lens, dtype, rows_of):
+def _prefill_reference(hq, hkv, d, total_q, q_lens, kv_lens, dtype, rows_of, window=None, sinks=0):
     """Shared body of the two prefill references (``reference.py:221-242,258-278``): per request
     with both lengths positive, its query rows attend its keys under the end-aligned causal mask;
     everything else stays 0 / -inf.  ``rows_of(r, kv_len, tensors)`` -> (K rows, V rows)."""
@@ -272,7 +284,7 @@ def _prefill_reference(hq, hkv, d, total_q, q_lens, kv_lens, dtype, rows_of):
             qs, qe = int(qo_indptr[r]), int(qo_indptr[r + 1])
             kk, vv = rows_of(r, int(kv_len), rest)
             o, l = _attend(q[qs:qe], kk.repeat_interleave(group, dim=1), vv.repeat_interleave(group, dim=1), sm_scale,
-                           causal_keep(int(q_len), int(kv_len), q.device))
+                           causal_keep(int(q_len), int(kv_len), q.device, window, sinks))
             out[qs:qe] = o.to(dtype)
             lse[qs:qe] = l
         return [out, lse]
@@ -280,7 +292,7 @@ def _prefill_reference(hq, hkv, d, total_q, q_lens, kv_lens, dtype, rows_of):
     return reference
 
 
-def gqa_paged_prefill_reference(dims, q_lens, kv_lens, dtype=None):
+def gqa_paged_prefill_reference(dims, q_lens, kv_lens, dtype=None, window=None, sinks=0):
     torch = _torch()
     hq, hkv, d, _pages, _n_idx, total_q = dims[:6]
 
@@ -290,10 +302,10 @@ def gqa_paged_prefill_reference(dims, q_lens, kv_lens, dtype=None):
         pages = kv_indices[base:base + kv_len].long()
         return k_cache[pages, 0], v_cache[pages, 0]
 
-    return _prefill_reference(hq, hkv, d, total_q, q_lens, kv_lens, dtype or torch.bfloat16, rows_of)
+    return _prefill_reference(hq, hkv, d, total_q, q_lens, kv_lens, dtype or torch.bfloat16, rows_of, window, sinks)
 
 
-def gqa_ragged_prefill_reference(dims, q_lens, kv_lens, dtype=None):
+def gqa_ragged_prefill_reference(dims, q_lens, kv_lens, dtype=None, window=None, sinks=0):
     torch = _torch()
     hq, hkv, d, total_q, _total_kv = dims[:5]
 
@@ -302,7 +314,7 @@ def gqa_ragged_prefill_reference(dims, q_lens, kv_lens, dtype=None):
         ks = int(kv_indptr[r])
         return k[ks:ks + kv_len], v[ks:ks + kv_len]
 
-    return _prefill_reference(hq, hkv, d, total_q, q_lens, kv_lens, dtype or torch.bfloat16, rows_of)
+    return _prefill_reference(hq, hkv, d, total_q, q_lens, kv_lens, dtype or torch.bfloat16, rows_of, window, sinks)
 
 
 # ----------------------------------------------------------------------------- MLA paged prefill

@@ -35,6 +35,8 @@ class DynamicOperator:
 
     def matches(self, attention) -> bool:
         a = attention
+        if a.window is not None or a.pages.shared is not None:        # (not an operator of this table, whatever its name)
+            return False
         if self.is_mla:
             return (a.is_mla and a.kind == self.spec.kind and a.page_size == self.page_size
                     and (a.num_qo_heads, a.head_dim, a.pe_dim) == tuple(self.dims[:3]))

@@ -311,10 +311,17 @@ _batch, _num_pages, _n_idx = cl.dims("batch num_pages n_idx", dynamic=True)
 _kv_len = cl.Dim("kv_len", dynamic=True, hint=4096)
 
 
-def paged_decode_op(hq=32, hkv=8, d=128, page=64, dtype=cl.f16, name=None):
+def _limits(window, sinks):
+    """The softmax arguments of a window and the name it gives an operator."""
+    return ({}, "") if window is None and not sinks else (dict(window=window, sinks=sinks), f"_w{window}_s{sinks}")
+
+
+def paged_decode_op(hq=32, hkv=8, d=128, page=64, dtype=cl.f16, name=None, window=None, sinks=0):
     """The paged GQA decode operator as a ``@jit`` program (the reference's registry form:
-    with a last-page-length input only when pages hold more than one token)."""
-    name = name or f"gqa_paged_decode_h{hq}_kv{hkv}_d{d}_ps{page}"
+    with a last-page-length input only when pages hold more than one token).  ``window``: the query sees the request's
+    last ``window`` keys and its first ``sinks`` ones."""
+    limits, suffix = _limits(window, sinks)
+    name = name or f"gqa_paged_decode_h{hq}_kv{hkv}_d{d}_ps{page}{suffix}"
 
     def body(q, k_cache, v_cache, pages):
         k, v = cl.paged_gather(k_cache, pages), cl.paged_gather(v_cache, pages)
@@ -325,13 +332,13 @@ def paged_decode_op(hq=32, hkv=8, d=128, page=64, dtype=cl.f16, name=None):
         def op(q, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, sm_scale):
             pages = cl.PageTable(kv_indptr, kv_indices, last_page_len=kv_last_page_len, length=_kv_len)
             qg, k, v = body(q, k_cache, v_cache, pages)
-            p, lse = cl.softmax((qg @ k.mT) * sm_scale, dim=-1, return_lse=True)
+            p, lse = cl.softmax((qg @ k.mT) * sm_scale, dim=-1, return_lse=True, **limits)
             return (p @ v).view(_batch, hq, d), lse.view(_batch, hq)
     else:
         def op(q, k_cache, v_cache, kv_indptr, kv_indices, sm_scale):
             pages = cl.PageTable(kv_indptr, kv_indices, length=_kv_len)
             qg, k, v = body(q, k_cache, v_cache, pages)
-            p, lse = cl.softmax((qg @ k.mT) * sm_scale, dim=-1, return_lse=True)
+            p, lse = cl.softmax((qg @ k.mT) * sm_scale, dim=-1, return_lse=True, **limits)
             return (p @ v).view(_batch, hq, d), lse.view(_batch, hq)
     # the annotations are built here rather than written on the signature: this module defers
     # annotation evaluation, and the extents are arguments of this factory
@@ -363,17 +370,48 @@ def mla_paged_decode_op(heads=16, ckv=512, kpe=64, dtype=cl.bf16, name=None):
     return cleave_amd.jit(name=name, dtype=dtype)(op)
 
 
+_n_shared = cl.Dim("n_shared", dynamic=True)
+
+
+def shared_prefix_decode_op(hq=32, hkv=8, d=128, page=64, dtype=cl.f16, name=None):
+    """Paged GQA decode of a batch whose requests all begin with the same pages (a system prompt, a document): their keys are read
+    once for the whole batch.  ``prefix_indices``: those pages, all of them full; ``kv_indptr`` / ``kv_indices`` /
+    ``kv_last_page_len``: each request's own pages behind them."""
+    name = name or f"gqa_shared_prefix_decode_h{hq}_kv{hkv}_d{d}_ps{page}"
+
+    def body(q, k_cache, v_cache, pages, sm_scale):
+        k, v = cl.paged_gather(k_cache, pages), cl.paged_gather(v_cache, pages)
+        p, lse = cl.softmax((q.view(_batch, hkv, hq // hkv, d) @ k.mT) * sm_scale, dim=-1, return_lse=True)
+        return (p @ v).view(_batch, hq, d), lse.view(_batch, hq)
+
+    if page > 1:
+        def op(q, k_cache, v_cache, prefix_indices, kv_indptr, kv_indices, kv_last_page_len, sm_scale):
+            pages = cl.PageTable(kv_indptr, kv_indices, last_page_len=kv_last_page_len, length=_kv_len, shared=prefix_indices)
+            return body(q, k_cache, v_cache, pages, sm_scale)
+    else:
+        def op(q, k_cache, v_cache, prefix_indices, kv_indptr, kv_indices, sm_scale):
+            return body(q, k_cache, v_cache, cl.PageTable(kv_indptr, kv_indices, length=_kv_len, shared=prefix_indices), sm_scale)
+    op.__annotations__ = {"q": cl.Tensor[_batch, hq, d], "k_cache": cl.Tensor[_num_pages, page, hkv, d],
+                          "v_cache": cl.Tensor[_num_pages, page, hkv, d], "prefix_indices": cl.Tensor[_n_shared, cl.i32],
+                          "kv_indptr": cl.Tensor[_batch + 1, cl.i32], "kv_indices": cl.Tensor[_n_idx, cl.i32],
+                          "sm_scale": cl.Scalar[cl.f32],
+                          **({"kv_last_page_len": cl.Tensor[_batch, cl.i32] | None} if page > 1 else {})}
+    return cleave_amd.jit(name=name, dtype=dtype)(op)
+
+
 _total_q, _total_kv = cl.dims("total_q total_kv", dynamic=True)
 _q_len = cl.Dim("q_len", dynamic=True)
 
 
-def prefill_op(hq=32, hkv=8, d=128, ragged=False, dtype=cl.bf16, name=None):
+def prefill_op(hq=32, hkv=8, d=128, ragged=False, dtype=cl.bf16, name=None, window=None, sinks=0):
     """The causal prefill operators as ``@jit`` programs (the reference's registry forms,
     ``demo/dynamic/gqa_paged_prefill.py`` / ``gqa_ragged_prefill.py``): ragged query rows per
-    request; keys through a token table, or packed per request."""
+    request; keys through a token table, or packed per request.  ``window``: a query sees the last ``window`` keys up to its
+    own and the first ``sinks`` ones of its request."""
     g = hq // hkv
+    limits, suffix = _limits(window, sinks)
     if ragged:
-        name = name or f"gqa_ragged_prefill_causal_h{hq}_kv{hkv}_d{d}"
+        name = name or f"gqa_ragged_prefill_causal_h{hq}_kv{hkv}_d{d}{suffix}"
 
         def op(q, k, v, qo_indptr, kv_indptr, sm_scale):
             rows = cl.PageTable(qo_indptr, length=_q_len)
@@ -381,14 +419,14 @@ def prefill_op(hq=32, hkv=8, d=128, ragged=False, dtype=cl.bf16, name=None):
             qr = cl.paged_gather(q, rows).view(_batch, hkv, g, _q_len, d)
             kr = cl.paged_gather(k, keys).view(_batch, hkv, 1, _kv_len, d)
             vr = cl.paged_gather(v, keys).view(_batch, hkv, 1, _kv_len, d)
-            p, lse = cl.softmax((qr @ kr.mT) * sm_scale, dim=-1, causal=True, return_lse=True)
+            p, lse = cl.softmax((qr @ kr.mT) * sm_scale, dim=-1, causal=True, return_lse=True, **limits)
             return (p @ vr).view(_total_q, hq, d), lse.view(_total_q, hq)
 
         op.__annotations__ = {"q": cl.Tensor[_total_q, hq, d], "k": cl.Tensor[_total_kv, hkv, d],
                               "v": cl.Tensor[_total_kv, hkv, d], "qo_indptr": cl.Tensor[_batch + 1, cl.i32],
                               "kv_indptr": cl.Tensor[_batch + 1, cl.i32], "sm_scale": cl.Scalar[cl.f32]}
     else:
-        name = name or f"gqa_paged_prefill_causal_h{hq}_kv{hkv}_d{d}_ps1"
+        name = name or f"gqa_paged_prefill_causal_h{hq}_kv{hkv}_d{d}_ps1{suffix}"
 
         def op(q, k_cache, v_cache, qo_indptr, kv_indptr, kv_indices, sm_scale):
             rows = cl.PageTable(qo_indptr, length=_q_len)
@@ -396,7 +434,7 @@ def prefill_op(hq=32, hkv=8, d=128, ragged=False, dtype=cl.bf16, name=None):
             qr = cl.paged_gather(q, rows).view(_batch, hkv, g, _q_len, d)
             k = cl.paged_gather(k_cache, pages).view(_batch, hkv, 1, _kv_len, d)
             v = cl.paged_gather(v_cache, pages).view(_batch, hkv, 1, _kv_len, d)
-            p, lse = cl.softmax((qr @ k.mT) * sm_scale, dim=-1, causal=True, return_lse=True)
+            p, lse = cl.softmax((qr @ k.mT) * sm_scale, dim=-1, causal=True, return_lse=True, **limits)
             return (p @ v).view(_total_q, hq, d), lse.view(_total_q, hq)
 
         op.__annotations__ = {"q": cl.Tensor[_total_q, hq, d], "k_cache": cl.Tensor[_num_pages, 1, hkv, d],

@@ -53,14 +53,19 @@ class PageTable:
     """A CSR table over requests.  With ``indices``: request ``r`` owns the pages
     ``indices[indptr[r]:indptr[r+1]]`` (and ``last_page_len[r]`` tokens of the last one; needed
     exactly when pages hold more than one token).  Without: the table is *ragged*, request ``r``
-    owns rows ``indptr[r]:indptr[r+1]`` of a packed tensor."""
+    owns rows ``indptr[r]:indptr[r+1]`` of a packed tensor.
 
-    def __init__(self, indptr, indices=None, last_page_len=None, length: Optional[Dim] = None):
+    ``shared``: pages that every request begins with, all of them full; a request's tokens are theirs, then those of its own
+    pages (which may be none)."""
+
+    def __init__(self, indptr, indices=None, last_page_len=None, length: Optional[Dim] = None, shared=None):
         if not (length is None or isinstance(length, Dim)):
             raise SpecError(f"PageTable(length=...) must be a cl.Dim, got {length!r}")
         if indices is None and last_page_len is not None:
             raise SpecError("PageTable: last_page_len needs indices (ragged rows have no pages)")
-        self.indptr, self.indices, self.last_page_len = indptr, indices, last_page_len
+        if indices is None and shared is not None:
+            raise SpecError("PageTable: shared pages need indices (ragged rows have no pages)")
+        self.indptr, self.indices, self.last_page_len, self.shared = indptr, indices, last_page_len, shared
         self.length = length if length is not None else Dim("kv_len", dynamic=True, hint=DEFAULT_KV_HINT)
 
     ragged = property(lambda self: self.indices is None)
@@ -88,15 +93,30 @@ def paged_gather(cache, pages: PageTable):
     return cache.program.apply("paged_gather", (cache,), pages=pages)
 
 
-def softmax(x, dim: int = -1, shift: Optional[float] = None, return_lse: bool = False, causal: bool = False):
+def _window_of(window, sinks):
+    """``(window, sinks)`` as whole numbers, or a ``SpecError``."""
+    for name, value, least in (("window", window, 1), ("sinks", sinks, 0)):
+        if value is not None and (isinstance(value, bool) or not isinstance(value, int) or value < least):
+            raise SpecError(f"softmax({name}=...) must be a whole number of at least {least}, got {value!r}")
+    if window is None and sinks:
+        raise SpecError("softmax(sinks=...) needs a window: without one every key before the query is visible")
+    return window, int(sinks or 0)
+
+
+def softmax(x, dim: int = -1, shift: Optional[float] = None, return_lse: bool = False, causal: bool = False,
+            window: Optional[int] = None, sinks: int = 0):
     """Softmax over ``dim``.  ``return_lse``: also the base-2 log of the sum of exponentials.
     ``causal``: scores are masked bottom-right aligned (query ``i`` sees keys ``j <= i + kv_len -
-    q_len``).  Both exist only in paged programs (and ``return_lse`` on torch tensors)."""
+    q_len``).  ``window``: a query sees the last ``window`` keys up to its own position only, and the first ``sinks`` keys of its
+    request (the one query of a decode program stands at the request's last key).  All exist only in paged programs (and
+    ``return_lse`` on torch tensors)."""
     traced = isinstance(x, Tensor)
+    window, sinks = _window_of(window, sinks)
     if traced and isinstance(x.program, PagedProgram):
-        return x.program.apply("softmax", (x,), dim=dim, return_lse=return_lse, causal=causal)
-    if causal or (traced and return_lse):
-        which = "causal=True" if causal else "return_lse=True"
+        return x.program.apply("softmax", (x,), dim=dim, return_lse=return_lse, causal=causal,
+                               **({"window": window, "sinks": sinks} if window is not None else {}))
+    if causal or window is not None or (traced and return_lse):
+        which = "causal=True" if causal else "window=..." if window is not None else "return_lse=True"
         raise SpecError(f"softmax({which}) is only lowerable inside a paged program")
     if not return_lse:
         return composites.softmax(x, dim, shift)
@@ -190,6 +210,8 @@ class PagedProgram(Recorder):
         for column in pages.columns():
             if column is not None:
                 self._mine(column, "PageTable")
+        if pages.shared is not None:
+            self._mine(pages.shared, "PageTable")
         ranks = (2, 3) if pages.ragged else (3, 4)
         if cache.ndim not in ranks:
             layout = "(total[, heads], d)" if pages.ragged else "(num_pages, page_size[, heads], d)"
@@ -217,13 +239,13 @@ class PagedProgram(Recorder):
         axis = dim % a.ndim
         return self.emit("reduce_sum", [a.id], [(a.dims[:axis] + (1,) + a.dims[axis + 1:], a.dtype)], dim=axis)
 
-    def _op_softmax(self, x, dim, return_lse, causal):
+    def _op_softmax(self, x, dim, return_lse, causal, **limits):
         self._mine(x, "softmax")
         axis = dim % x.ndim
         results = [(x.dims, x.dtype)]
         if return_lse:
             results.append((x.dims[:axis] + x.dims[axis + 1:], f32))
-        return self.emit("softmax", [x.id], results, dim=axis, causal=bool(causal))
+        return self.emit("softmax", [x.id], results, dim=axis, causal=bool(causal), **limits)
 
     def attention(self) -> "PagedAttention":
         return PagedAttention.recognize(self)
@@ -249,7 +271,8 @@ class PagedProgram(Recorder):
                     for op in self.oplist],
             "params": [{"name": p.name, "spec": spec_doc(p.spec), "value": p.value} for p in self.params],
             "tables": [{"indptr": column(t.indptr), "indices": column(t.indices),
-                        "last_page_len": column(t.last_page_len), "length": dim_to_doc(t.length)} for t in self.tables],
+                        "last_page_len": column(t.last_page_len), "length": dim_to_doc(t.length),
+                        **({"shared": column(t.shared)} if t.shared is not None else {})} for t in self.tables],
             "outputs": [[name, number] for name, number in self.outputs],
         }
 
@@ -277,7 +300,7 @@ class PagedProgram(Recorder):
 
         program.params = [Param(p["name"], spec_from(p["spec"]), p["value"]) for p in doc["params"]]
         program.tables = [PageTable(column(t["indptr"]), column(t["indices"]), column(t["last_page_len"]),
-                                    dim_from_doc(t["length"])) for t in doc["tables"]]
+                                    dim_from_doc(t["length"]), column(t.get("shared"))) for t in doc["tables"]]
         program.outputs = [(name, number) for name, number in doc["outputs"]]
         return program
 
@@ -369,11 +392,13 @@ class PagedAttention:
     GQA ``softmax((q @ gather(K).mT) * scale) @ gather(V)`` and
     MLA ``softmax((qn @ gather(CKV).mT + qp @ gather(KPE).mT) * scale) @ gather(CKV)``,
     each optionally with the lse as a second output.  A prefill gathers its queries through
-    ragged rows and masks causally."""
+    ragged rows and masks causally.  A softmax may carry a ``window`` (and ``sinks``); a decode's page table may have pages that
+    all requests share."""
 
-    def __init__(self, program, queries, caches, pages, scale, out, lse=None, rows=None, causal=False):
+    def __init__(self, program, queries, caches, pages, scale, out, lse=None, rows=None, causal=False, window=None, sinks=0):
         self.program, self.queries, self.caches = program, tuple(queries), tuple(caches)
         self.pages, self.scale, self.out, self.lse, self.rows, self.causal = pages, scale, out, lse, rows, bool(causal)
+        self.window, self.sinks = window, int(sinks or 0)
 
     @classmethod
     def recognize(cls, program: PagedProgram) -> "PagedAttention":
@@ -441,7 +466,8 @@ class PagedAttention:
             if len(weights.what.outs) != 2 or through != weights.what.outs[1]:
                 refuse("the second output must be the softmax's lse")
         return cls(program, [q for q, _, _ in parts], caches[:2], program.tables[table], factors[0].what, out_number,
-                   lse_number, None if rows is None else program.tables[rows], weights.what.attr("causal"))
+                   lse_number, None if rows is None else program.tables[rows], weights.what.attr("causal"),
+                   weights.what.attr("window"), weights.what.attr("sinks", 0))
 
     # ---------------------------------------------------------------- facts about the operator
     is_mla = property(lambda self: len(self.queries) == 2)
@@ -469,6 +495,10 @@ class PagedAttention:
             raise SpecError(f"{name}: ragged (unpaged) KV is only built for prefill")
         if self.is_mla and self.pages.ragged:
             raise SpecError(f"{name}: MLA reads a paged cache; ragged MLA is not built")
+        if self.is_mla and (self.window is not None or self.pages.shared is not None):
+            raise SpecError(f"{name}: a window and shared pages are built for GQA, not for MLA")
+        if self.pages.shared is not None and (self.is_prefill or self.window is not None):
+            raise SpecError(f"{name}: shared pages are built for decode, without a window")
         layer = {
             (True, True): kinds.MLA_PAGED_PREFILL_CAUSAL, (True, False): kinds.MLA_PAGED_DECODE,
             (False, True): kinds.RAGGED_PREFILL_CAUSAL if self.pages.ragged else kinds.PAGED_PREFILL_CAUSAL,
@@ -545,6 +575,13 @@ class PagedAttention:
             said["last_page_len_input"] = last.kernel_name
         elif last is not None and (self.is_mla or not last.spec.optional):
             raise SpecError(f"{name} reads no last_page_len; drop it or make it optional")
+        if self.window is not None:
+            said.update(window=self.window, sinks=self.sinks)
+        if self.pages.shared is not None:
+            shared = self._param_of(self.pages.shared)
+            if shared is None or len(shared.spec.dims) != 1:
+                raise SpecError(f"{name}: the shared pages are a vector argument of page numbers")
+            said.update(shared_input=shared.kernel_name, shared_dim=axis(shared))
         nameless = [field for field, value in said.items() if value is None]
         if nameless:
             raise SpecError(f"{name}: {nameless} must be named cl.Dims")
@@ -583,10 +620,13 @@ class PagedDecodeWorkloads:
     """Synthetic decode workloads: every ``batch`` size times ``samples`` kv lengths spread
     geometrically over ``kv_len``.  In a workload the first request has the full length and the
     others are uniform in [length / 2, length], drawn from a generator seeded by the CRC-32 of
-    ``repr((seed, batch, length))`` (``python/cleave/frontend/paged.py:575-618``)."""
+    ``repr((seed, batch, length))`` (``python/cleave/frontend/paged.py:575-618``).  ``prefix``: tokens
+    of the pages that the requests of an operator with shared pages begin with (rounded up to whole pages; other
+    operators have none); ``kv_len`` counts the tokens behind them."""
 
-    def __init__(self, batch=(1, 7, 64), kv_len=(1, 8192), samples: int = 3, seed: int = 0):
+    def __init__(self, batch=(1, 7, 64), kv_len=(1, 8192), samples: int = 3, seed: int = 0, prefix: int = 2048):
         self.batch, self.kv_len, self.samples, self.seed = tuple(batch), tuple(kv_len), int(samples), int(seed)
+        self.prefix = int(prefix)
 
     def __repr__(self):
         return f"cl.workloads.paged_decode(batch={self.batch}, kv_len={self.kv_len}, samples={self.samples}, seed={self.seed})"
@@ -612,18 +652,70 @@ class PagedDecodeWorkloads:
         page, dtype = attention.page_size, attention.program.dtype.torch
         heads = (attention.num_qo_heads, attention.num_kv_heads, attention.head_dim)
         axes = sampled(self.axes(), keep)
+        shared = math.ceil(self.prefix / page) if attention.pages.shared is not None else 0
+        limits = {"window": attention.window, "sinks": attention.sinks, "shared": shared}
 
         def generate():
             for batch, length in axes:
                 lens = self.lengths(batch, length)
                 pages = sum(math.ceil(n / page) for n in lens)
-                dims = (batch, *heads, pages, pages)
-                inputs = reference.gqa_paged_decode_inputs(dims, lens, page_size=page, dtype=dtype)
-                expected = reference.gqa_paged_decode_reference(dims, lens, page_size=page, dtype=dtype)(*inputs)
+                dims = (batch, *heads, pages + shared, pages)
+                inputs = reference.gqa_paged_decode_inputs(dims, lens, page_size=page, dtype=dtype, shared=shared)
+                expected = reference.gqa_paged_decode_reference(dims, lens, page_size=page, dtype=dtype, **limits)(*inputs)
                 yield workload_key((batch, length)), inputs, expected
+
+        return generate
+
+
+class CausalPrefillWorkloads:
+    """Synthetic prompts for a GQA causal prefill: every ``batch`` size times ``samples`` numbers of new tokens spread
+    geometrically over ``q_len``, the first request with all of them and the others uniform in [length / 2, length]; ``prefix``: the
+    range of keys a request already has in its cache, uniform too.  Drawn as ``PagedDecodeWorkloads`` draws."""
+
+    def __init__(self, batch=(1, 8), q_len=(1, 2048), prefix=(0, 1024), samples: int = 3, seed: int = 0):
+        self.batch, self.q_len, self.prefix = tuple(batch), tuple(q_len), tuple(prefix)
+        self.samples, self.seed = int(samples), int(seed)
+
+    def __repr__(self):
+        return (f"cl.workloads.causal_prefill(batch={self.batch}, q_len={self.q_len}, prefix={self.prefix}, samples={self.samples}, "
+                f"seed={self.seed})")
+
+    def axes(self) -> list:
+        return PagedDecodeWorkloads(self.batch, self.q_len, self.samples).axes()
+
+    def lengths(self, batch: int, q_len: int):
+        """``(new tokens, keys)`` of every request."""
+        draw = random.Random(zlib.crc32(repr((self.seed, batch, q_len)).encode()))
+        floor = max(self.q_len[0], q_len // 2)
+        new = [q_len] + [draw.randint(floor, q_len) for _ in range(batch - 1)]
+        return new, [n + draw.randint(*self.prefix) for n in new]
+
+    def factory(self, attention: PagedAttention, keep: int = 0):
+        from ..dynamic import reference
+        from ..runtime.autotune import sampled, workload_key
+
+        if attention.is_mla or not attention.is_prefill:
+            raise SpecError(f"{attention.program.name}: cl.workloads.causal_prefill makes prompts of a GQA causal prefill")
+        dtype = attention.program.dtype.torch
+        heads = (attention.num_qo_heads, attention.num_kv_heads, attention.head_dim)
+        axes = sampled(self.axes(), keep)
+        limits = {"window": attention.window, "sinks": attention.sinks}
+
+        def generate():
+            for batch, q_len in axes:
+                new, keys = self.lengths(batch, q_len)
+                if attention.pages.ragged:
+                    dims = (*heads, sum(new), sum(keys))
+                    make, refer = reference.gqa_ragged_prefill_inputs, reference.gqa_ragged_prefill_reference
+                else:
+                    dims = (*heads, sum(keys), sum(keys), sum(new))
+                    make, refer = reference.gqa_paged_prefill_inputs, reference.gqa_paged_prefill_reference
+                inputs = make(dims, new, keys, dtype=dtype)
+                yield workload_key((batch, q_len)), inputs, refer(dims, new, keys, dtype=dtype, **limits)(*inputs)
 
         return generate
 
 
 class workloads:  # noqa: N801  (spelled ``cl.workloads.paged_decode(...)``)
     paged_decode = PagedDecodeWorkloads
+    causal_prefill = CausalPrefillWorkloads

@@ -114,7 +114,7 @@ def schedule_paged(graphs, spec, config, *, split_graphs=(), filter_before_topk=
                 # split / these: 64 requests, 68237 tokens 66 / 41.6, 40 of up to 4000 91 / 66, 23 of 2682 40 / 28.8, 18 of 1056 16.2 / 14.9;
                 # behind the fixed split for four requests and fewer, 3 of 2882 11.5 / 12.9, which keep it by the calibrated rule, and the single
                 # kernel for short ones, 63 of 50 8.1 / 10.5)
-                if (getattr(spec, "page_size", 1) == 1 or spec.page_size >= 16) and single.dense.query_rows <= 16 and factor == max(factors):
+                if getattr(spec, "window", None) is None and (getattr(spec, "page_size", 1) == 1 or spec.page_size >= 16) and single.dense.query_rows <= 16 and factor == max(factors):
                     forms.append(dataclasses.replace(single.dense, chunk_pages=-1, lockstep=True, waves=spec.num_kv_heads,
                                                      n_threads=spec.num_kv_heads * 64))
             for d in forms:
@@ -243,13 +243,15 @@ def calibrate_dispatch(pair, solo, factory, spec, fixed=None) -> dict:
     pair, solo = dataclasses.replace(pair, latency_us={}), dataclasses.replace(solo, latency_us={})
     indptr_at = param_index(solo.kernel, f"PlaceHolder_{spec.indptr_input}")
     tokens_per_unit, kv_tile = int(getattr(spec, "page_size", 1)), int(pair.tiling.kv_tile)
+    # (of a window, a request's tiles are those it sees)
+    seen = None if getattr(spec, "window", None) is None else spec.window + spec.sinks
     longest, requests = {}, {}
 
     def observed():
         for key, inputs, expected in factory(0)():
             bounds = inputs[indptr_at].tolist()
-            units = max(hi - lo for lo, hi in zip(bounds, bounds[1:]))
-            longest[key], requests[key] = math.ceil(units * tokens_per_unit / kv_tile), len(bounds) - 1
+            tokens = max(hi - lo for lo, hi in zip(bounds, bounds[1:])) * tokens_per_unit
+            longest[key], requests[key] = math.ceil(min(tokens, seen or tokens) / kv_tile), len(bounds) - 1
             yield key, inputs, expected
 
     def alone():
@@ -278,7 +280,7 @@ def calibrate_dispatch(pair, solo, factory, spec, fixed=None) -> dict:
         "rule": "run the split pair when the longest request has at least min_tiles KV tiles (lone_tiles for batches of fewer "
                 "than few_requests requests; indptr units x page_size tokens / kv_tile), else the single kernel",
         "min_tiles": min_tiles, "lone_tiles": lone_tiles, "few_requests": few, "kv_tile": kv_tile,
-        "page_size": tokens_per_unit, "indptr_index": indptr_at,
+        "page_size": tokens_per_unit, "indptr_index": indptr_at, **({"seen_tokens": seen} if seen else {}),
         "split_label": pair.label, "single_label": solo.label,
         "n_workloads": len(keys), "split_runs": sum(map(splits, keys)),
         "geomean_us": {"hybrid": geomean(list(per_workload.values())), "split": geomean([pair.latency_us[k] for k in keys]),
@@ -495,7 +497,7 @@ class PagedKernel(Kernel):
             raise CleaveError(f"{self.name}: no split / single calibration was made (or saved) for this operator")
         few = requests is not None and requests < rule.get("few_requests", 0)
         # (tiles of the longest request, rounded up, against a whole number of them)
-        tokens, kv_tile = int(longest) * rule["page_size"], rule["kv_tile"]
+        tokens, kv_tile = min(int(longest) * rule["page_size"], rule.get("seen_tokens", 1 << 62)), rule["kv_tile"]
         if tokens <= (rule["lone_tiles" if few else "min_tiles"] - 1) * kv_tile:
             return "single"
         if requests is not None and "fixed" in sources and "fixed" in rule:
