@@ -601,6 +601,33 @@ class HipCodeGen:
             else:
                 self._launch_combine(unit, total_rows, p["vdim"], splits, plain=plain)
 
+    def _emit_attn_shared(self, unit, plan, params, partial, combine, fused):
+        """Decode over shared pages and the requests' own: one launch for both kinds of work, and the sum of their partials."""
+        p, op = plan.problem, plan.operands
+        d, group = p["head_dim"], p["group"]
+        if plan.role != "main" or d % 64 or d > 256 or not (d == 64 or d % 128 == 0):
+            raise CodegenError("attention over shared pages is one unsplit operator, of heads 64, 128 or 256 wide")
+        batch, ranges = p["dim_names"]["batch"], "(prefix_ranges + own_ranges)"
+        rows = f"({batch} * {p['q_heads']})"
+        plan = dataclasses.replace(plan, role="fused", split_factor=2)
+        self._attn_common(unit, plan, params, True, True, False, d, f"(batch * {p['q_heads']})", bool(p["emit_lse"]))
+        unit.define("CL_ITEM_RANGES", ranges)
+        by_name = self._by_name(params)
+        names = [q.name for q in params if q.role in ("input", "scalar")] + [op[r] for r in ("PM", "PL", "PO")]
+        unit.define("CL_PARTIAL_ARGS", ", ".join([by_name[n].name for n in names] + list(p["dim_names"]) + [n for n, _ in plan.extra["derived_dims"]]))
+        for k, v in (("CL_PREFIX", 1), ("CL_OWN_PART", 1), ("CL_RAGGED", 0), ("CL_HEAD_DIM", d), ("CL_KV_HEADS", p["kv_heads"]),
+                     ("CL_Q_HEADS", p["q_heads"]), ("CL_ROWS", group), ("CL_WAVES", 4), ("CL_PREFETCH", 1), ("CL_PAGED", 1),
+                     ("CL_PAGE_SIZE", p["page_size"])):
+            unit.define(k, v)
+        for role in ("Q", "K", "V", "SHARED", "INDPTR", "INDICES", "LAST"):
+            if role in op:
+                unit.define(f"CL_ARG_{role}", op[role])
+        unit.templates += ["attn_tile.hip", "attn_prefill_lds.hip", "attn_decode.hip", "attn_shared.hip", "attn_combine.hip"]
+        prefix = f"ceildiv({p['kv_heads']} * prefix_ranges, 8) * 8 * ceildiv({batch} * {group}, 128)"
+        own = f"{batch} * {p['kv_heads'] * -(-group // 16)} * own_ranges"
+        unit.launch(ENTRY, (f"{prefix} + {own}", 1, 1), 256, 0, self._partial_args)
+        self._launch_chunk_combine(unit, rows, d, f"{batch} * {ranges}")
+
     def _emit_attn_dense_prefill(self, unit, plan, params, partial, combine):
         """The LDS-shared prefill kernel over the dense attention family's operands: every unit
         (batch entry x kv head) has ``group * sq`` query rows that all see all keys."""

@@ -4,6 +4,13 @@
 #ifndef CL_CHUNK_PAGES
 #define CL_CHUNK_PAGES 0
 #endif
+// CL_ITEM_RANGES: items are not cut from a page table; every request has that many (a run-time expression), one behind the other
+#ifndef CL_ITEM_RANGES
+#define CL_ITEM_RANGES 0
+#define CB_FIXED_ITEMS 0
+#else
+#define CB_FIXED_ITEMS 1
+#endif
 #ifndef CL_PO_ELEM
 #define CL_PO_ELEM 0
 #endif
@@ -62,7 +69,7 @@ CL_DEVICE void cb_finish(float m, float l, f32x4 o, elem_t* out, float* lse) {
   cb_store(top, l, o, out, lse);
 }
 #endif
-#if CL_CHUNK_PAGES && CL_EMIT_COMBINE
+#if (CL_CHUNK_PAGES || CB_FIXED_ITEMS) && CL_EMIT_COMBINE
 // Combine of chunked items: request b owns items b + p0/C .. b + (p1-1)/C (p0, p1 its page-table range); partials are (item,
 // query head[, d]).  Every load of a round of items is issued before the first use (the trip count is a run-time value: left alone,
 // each item's loads wait for the previous item's); the running maximum is carried along and the sums rescaled when a round raises
@@ -79,18 +86,24 @@ CL_DEVICE void cb_finish(float m, float l, f32x4 o, elem_t* out, float* lse) {
 // the 2048 workgroups of 32 latent requests of up to 1000 keys took 18.6 us where these take 18.0.  Eight items a round spill.)
 extern "C" __global__ void __launch_bounds__(256, 8)
 CL_COMBINE_NAME(CL_COMBINE_PARAMS) {
+#if !CB_FIXED_ITEMS
   asm volatile("" :: "s"(CL_CARG_INDPTR), "s"(CL_CARG_PM), "s"(CL_CARG_PL), "s"(CL_CARG_PO), "s"(CL_CARG_OUT), "s"(n_idx), "s"(chunk_pages), "s"(batch), "s"(gridDim.x));
+#endif
   float m = CL_NEG_BIG, l = 0.f;
   f32x4 o = (f32x4){0.f, 0.f, 0.f, 0.f};
   // items `from`, from + STEP, .. of a row, EACH of them at a time; the last round begins where one is missing to a thread `ahead` of this
   auto add_up = [&](auto each, auto step, const i64 row, const int d, const int from, const int ahead) __attribute__((always_inline)) {
     constexpr int EACH = decltype(each)::value, STEP = decltype(step)::value;
     const int req = (int)(row / CL_Q_HEADS), qh = (int)(row % CL_Q_HEADS);
+#if CB_FIXED_ITEMS
+    const int count = CL_ITEM_RANGES, first = req * count;
+#else
     int p0 = CL_CARG_INDPTR[req], p1 = CL_CARG_INDPTR[req + 1];
     p0 = p0 < 0 ? 0 : (p0 > n_idx ? n_idx : p0);
     p1 = p1 < 0 ? 0 : (p1 > n_idx ? n_idx : p1);
     const int first = req + p0 / chunk_pages;
     const int count = p1 > p0 ? (p1 - 1) / chunk_pages - p0 / chunk_pages + 1 : 0;
+#endif
     auto round = [&](auto whole, const int s) __attribute__((always_inline)) {
       constexpr int WHOLE = decltype(whole)::value;
       float pm[EACH], pl[EACH];

@@ -41,7 +41,21 @@
 //                numbered without the ones in between (step s is 32-token step s of the request up to the sinks' last one and
 //                s + skip behind it), so that splits share out what is seen; the ragged edges are masked.
 
+//   CL_OWN_PART  paged: not a kernel but the device function att_own_part(arguments, block) of attn_shared.hip: the requests' own keys
+//                behind pages that they share, cut into `own_ranges` (a run-time argument) parts whose partials lie behind those
+//                of the shared keys
+
 #define ATT_RAISE_BY 8.0f
+#ifndef CL_OWN_PART
+#define CL_OWN_PART 0
+#endif
+#if CL_OWN_PART
+#define ATT_SPLITS own_ranges
+#define ATT_PROW(split, orow) ((((orow) / CL_Q_HEADS) * (prefix_ranges + own_ranges) + prefix_ranges + (split)) * CL_Q_HEADS + (orow) % CL_Q_HEADS)
+#else
+#define ATT_SPLITS CL_SPLITS
+#define ATT_PROW(split, orow) ((i64)(split) * CL_TOTAL_ROWS + (orow))
+#endif
 #ifndef CL_WINDOW
 #define CL_WINDOW 0
 #endif
@@ -201,13 +215,23 @@ CL_DEVICE int att_clamp_ptr(int p, int n_idx) { return p < 0 ? 0 : (p > n_idx ? 
 #else
 #define ATT_WAVES_PER_SIMD 1
 #endif
+#if CL_OWN_PART
+CL_DEVICE void att_own_part(CL_PARTIAL_PARAMS, const int block) {
+#else
 extern "C" __global__ void __launch_bounds__(CL_WAVES * 64, ATT_WAVES_PER_SIMD)
 CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
+#endif
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int c = lane & 15, g = lane >> 4;
 #if CL_CHUNK_PAGES
   const int split = 0, tile_id = 0;
   const int item = blockIdx.x;
+#elif CL_OWN_PART
+  // (as a grid of (units, ranges) is laid out)
+  const int split = block / (batch * CL_KV_HEADS * ATT_ROW_TILES);
+  const int unit_tile = block % (batch * CL_KV_HEADS * ATT_ROW_TILES);
+  const int tile_id = unit_tile % ATT_ROW_TILES;
+  const int unit = unit_tile / ATT_ROW_TILES;
 #else
   const int split = blockIdx.y;
 #if CL_SKEW
@@ -273,7 +297,11 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
   // CSR: every page but the last is full, the last holds kv_last_page_len tokens, and the
   // sum is clamped to the pages the request owns.
   const int req = unit / CL_KV_HEADS, head = unit % CL_KV_HEADS;
+#if CL_WINDOW || CL_OWN_PART
+  const int p0 = cl_clamp_ptr(CL_ARG_INDPTR[req], n_idx), p1 = cl_clamp_ptr(CL_ARG_INDPTR[req + 1], n_idx);
+#else
   const int p0 = CL_ARG_INDPTR[req], p1 = CL_ARG_INDPTR[req + 1];
+#endif
   int n_pages = p1 - p0;
   n_pages = n_pages > 0 ? n_pages : 0;
   {
@@ -345,7 +373,7 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
     step_end = (split & 1) == 0 ? lo + first : hi;
   }
 #else
-  const int per_split = (n_steps + CL_SPLITS - 1) / CL_SPLITS;
+  const int per_split = (n_steps + ATT_SPLITS - 1) / ATT_SPLITS;
   const int step_begin = split * per_split;
   int step_end = step_begin + per_split;
   step_end = step_end < n_steps ? step_end : n_steps;
@@ -488,7 +516,11 @@ _Pragma("unroll")                                                               
   // per lane and accumulator: whole 1 KiB rows), and the first wave folds them into its own by the
   // max-rescale rule: one LDS round trip for all of them --------------------------------------
   {
+#if CL_OWN_PART
+    float* att_lds = reinterpret_cast<float*>(pl_tiles);                      // (the shared keys' images: this workgroup has none)
+#else
     extern __shared__ float att_lds[];
+#endif
     f32x4* sh_o = reinterpret_cast<f32x4*>(att_lds);                          // [WAVES - 1][8 ATT_VC][64]
     float* sh_m = att_lds + (CL_WAVES - 1) * 8 * ATT_VC * 64 * 4;              // [WAVES - 1][16]
     float* sh_l = sh_m + (CL_WAVES - 1) * 16;                                  // [WAVES - 1][16]
@@ -539,7 +571,7 @@ _Pragma("unroll")                                                               
     float* dst = CL_ARG_PO + prow * CL_VDIM;
     (void)orow;
 #elif CL_SPLITS > 1
-    const i64 prow = (i64)split * CL_TOTAL_ROWS + orow;
+    const i64 prow = ATT_PROW(split, orow);
     float* dst = CL_ARG_PO + prow * CL_VDIM;
 #else
     elem_t* dst = CL_ARG_OUT + orow * CL_VDIM;

@@ -57,6 +57,10 @@
 // registers); the lanes on the diagonal take the reciprocal root and the lanes of each score
 // fetch the factor of its key.
 //
+// CL_PREFIX: not a kernel but the device function pl_prefix_part(arguments, block) of attn_shared.hip: the pages that all requests of
+// a decode begin with.  The rows are the whole batch's, `batch` tokens of CL_Q_HEADS heads, all of them seeing all keys; the keys are
+// cut into `prefix_ranges` (a run-time argument), each walked by one workgroup per kv head and 128 rows that writes f32 partials.
+//
 // CL_PF_XCD / CL_PF_REVERSE (default 1) switch the XCD mapping and the walking order.
 //
 // CL_WINDOW, CL_SINKS (paged modes): a row sees the last CL_WINDOW keys up to its own and the request's first CL_SINKS ones.
@@ -90,6 +94,9 @@
 #ifndef CL_KNORM
 #define CL_KNORM 0
 #endif
+#ifndef CL_PREFIX
+#define CL_PREFIX 0
+#endif
 #ifndef CL_WINDOW
 #define CL_WINDOW 0
 #define CL_SINKS 0
@@ -100,8 +107,19 @@
 #if CL_DENSE && !CL_RAGGED
 #error "dense operands have consecutive key rows (CL_RAGGED)"
 #endif
-#if CL_SPLITS > 1 && !CL_DENSE
-#error "split keys: dense operands only"
+#if CL_SPLITS > 1 && !CL_DENSE && !CL_PREFIX
+#error "split keys: dense operands and shared pages only"
+#endif
+#if CL_PREFIX
+#define PL_TABLE CL_ARG_SHARED
+#define PL_PROW(split, m) ((((i64)(lo + (m)) / PL_GROUP) * (prefix_ranges + own_ranges) + (split)) * CL_Q_HEADS + head * PL_GROUP + (lo + (m)) % PL_GROUP)
+#define PL_PAGE(pos) ((pos) / CL_PAGE_SIZE)
+#define PL_ROW(page, pos) ((page) * CL_PAGE_SIZE + (pos) % CL_PAGE_SIZE)
+#else
+#define PL_TABLE CL_ARG_INDICES
+#define PL_PROW(split, m) ((i64)(split) * CL_TOTAL_ROWS + row_index(m))
+#define PL_PAGE(pos) (pos)
+#define PL_ROW(page, pos) (page)
 #endif
 #define PL_STEP 32
 #define PL_GROUP (CL_Q_HEADS / CL_KV_HEADS)
@@ -121,19 +139,29 @@
 #define PL_KJ (CL_HEAD_DIM / 32)
 #define PL_FB (CL_VDIM / 16)
 #define PL_UNITS_PER (PL_KPANELS + PL_VPANELS)   // 1 KiB loads per wave and step: its 8-key group of every panel of K and V
-static_assert(CL_Q_HEADS % CL_KV_HEADS == 0 && 16 % PL_GROUP == 0, "the head group divides the 16-row query tile");
+static_assert(CL_Q_HEADS % CL_KV_HEADS == 0 && (CL_PREFIX || 16 % PL_GROUP == 0), "the head group divides the 16-row query tile");
 static_assert(CL_HEAD_DIM % 64 == 0 && CL_HEAD_DIM <= 256 && CL_VDIM % 64 == 0 && CL_VDIM <= 256,
               "key and value widths in whole 64-feature panels");
 static_assert(PL_UNITS_PER < 16, "load counter range");
 
+#if CL_PREFIX
+// (the workgroups of the other part merge their waves here: 8 KiB and 128 bytes of each but the first per 128 value features)
+#define PL_MERGE (3 * ((CL_VDIM + 127) / 128 * 4096 + 64))
+__shared__ __attribute__((aligned(1024))) elem_t pl_tiles[PL_STAGES * PL_STAGE > PL_MERGE ? PL_STAGES * PL_STAGE : PL_MERGE];
+#else
 __shared__ __attribute__((aligned(1024))) elem_t pl_tiles[PL_STAGES * PL_STAGE];
+#endif
 #if !CL_RAGGED
 __shared__ __attribute__((aligned(256))) int pl_ids[2][4][64];   // table entries on their way in: [step parity][wave][lane]
 #endif
 
 #if CL_EMIT_PARTIAL
+#if CL_PREFIX
+CL_DEVICE void pl_prefix_part(CL_PARTIAL_PARAMS, const int block) {
+#else
 extern "C" __global__ void __launch_bounds__(256, 2)
 CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
+#endif
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
   // Workgroups go to the 8 XCDs round-robin in launch order; every XCD has its own L2.  XCD x
@@ -142,6 +170,16 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
   // the same keys out of that L2.  Heaviest first: within a request later items see more keys, so
   // every eighth is walked backwards.
   int item, head;
+#if CL_PREFIX
+  // The row tiles that walk one kv head's range of keys run next to each other on one XCD and share the keys out of its L2: XCD x
+  // takes every eighth (range, kv head) pair, all of a pair's tiles before the next.
+  const int row_tiles = (batch * PL_GROUP + PL_ROWS - 1) / PL_ROWS;
+  const int pair = block / 8 / row_tiles * 8 + block % 8;
+  item = block / 8 % row_tiles;
+  head = pair % CL_KV_HEADS;
+  const int split = pair / CL_KV_HEADS;
+  if (split >= prefix_ranges) return;                   // (the pairs are padded to a multiple of eight)
+#else
   {
     const int gx = (int)gridDim.x, launch = (int)blockIdx.x + gx * (int)blockIdx.y;
 #if CL_PF_XCD
@@ -156,7 +194,22 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
     item = lin % gx;
     head = lin / gx;
   }
-#if CL_DENSE
+#endif
+#if CL_PREFIX
+  const int lo = item * PL_ROWS;
+  const int n_rows = batch * PL_GROUP - lo < PL_ROWS ? batch * PL_GROUP - lo : PL_ROWS;
+  const int all_keys = n_shared * CL_PAGE_SIZE;
+  const int per_range = ((all_keys + PL_STEP - 1) / PL_STEP + prefix_ranges - 1) / prefix_ranges * PL_STEP;
+  const int kv0 = split * per_range;                    // this range's first key
+  int n_keys = all_keys - kv0 < per_range ? all_keys - kv0 : per_range;
+  n_keys = n_keys > 0 ? n_keys : 0;
+  const int q0 = 0, off = 0, ext = n_keys;
+  (void)q0; (void)off;
+  auto row_index = [&](int m) __attribute__((always_inline)) {
+    return (i64)((lo + m) / PL_GROUP) * CL_Q_HEADS + head * PL_GROUP + (lo + m) % PL_GROUP;
+  };
+  auto row_limit = [&](int m) __attribute__((always_inline)) { (void)m; return n_keys - 1; };
+#elif CL_DENSE
   // dense operands: `head` is a unit (batch entry x kv head) with CL_ROWS query rows (its head group
   // x the query positions, all seeing all CL_SKV keys); an item is 128 consecutive rows of them
   const int lo = item * PL_ROWS;
@@ -214,7 +267,7 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
 #pragma unroll
     for (int rt = 0; rt < 2; ++rt) {
       if (!live[rt]) continue;
-      const i64 prow = (i64)split * CL_TOTAL_ROWS + orow[rt];
+      const i64 prow = PL_PROW(split, 32 * wave + 16 * rt + c);
       float* dstp = CL_ARG_PO + prow * CL_VDIM + 4 * g;
 #pragma unroll
       for (int fb = 0; fb < PL_FB; ++fb) *reinterpret_cast<f32x4*>(dstp + 16 * fb) = (f32x4){0.f, 0.f, 0.f, 0.f};
@@ -332,16 +385,19 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
   auto key_pos = [&](int s) __attribute__((always_inline)) {
     return PL_STEP * tile_of(s < last_step ? s : last_step) + (s < last_step ? my_r : row_tail);
   };
-  auto row_of = [&](int s) __attribute__((always_inline)) { return pl_clamp(CL_ARG_INDICES[kv0 + key_pos(s)], 0, num_pages - 1); };
+  auto row_of = [&](int s) __attribute__((always_inline)) {
+    const int at = kv0 + key_pos(s);
+    return PL_ROW(pl_clamp(PL_TABLE[PL_PAGE(at)], 0, num_pages - 1), at);
+  };
   // In the loop the lane's table entry travels like the tiles do, global -> LDS on the kernel's
   // own load counter, a step ahead of the loads that need it (a load the compiler tracks would
   // make it wait for every load in flight): entry of step s into pl_ids[s & 1][wave][lane].
   const unsigned ids_byte = (unsigned)(size_t)(__attribute__((address_space(3))) int*)&pl_ids[0][0][0];
   auto fetch_id = [&](int s) __attribute__((always_inline)) {
-    pl_dma4(CL_ARG_INDICES + kv0 + key_pos(s), ids_byte + (unsigned)(((s & 1) * 4 + wave) * 256));
+    pl_dma4(PL_TABLE + PL_PAGE(kv0 + key_pos(s)), ids_byte + (unsigned)(((s & 1) * 4 + wave) * 256));
   };
   auto fetched_row = [&](int s) __attribute__((always_inline)) {
-    return pl_clamp(pl_ids[s & 1][wave][lane], 0, num_pages - 1);
+    return PL_ROW(pl_clamp(pl_ids[s & 1][wave][lane], 0, num_pages - 1), kv0 + key_pos(s));
   };
 #endif
 
@@ -767,7 +823,7 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
 #if CL_SPLITS > 1
     // split partials: unnormalised f32 values (16 bytes per lane and block), m and l by the g == 0 lanes
     {
-      const i64 prow = (i64)split * CL_TOTAL_ROWS + orow;
+      const i64 prow = PL_PROW(split, m);
       float* dstp = CL_ARG_PO + prow * CL_VDIM + 4 * g_e;
 #pragma unroll
       for (int fb = 0; fb < PL_FB; ++fb) *reinterpret_cast<f32x4*>(dstp + 16 * fb) = acc[rt][fb];

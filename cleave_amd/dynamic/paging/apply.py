@@ -137,7 +137,7 @@ def read_dense_combine(plan: KernelPlan) -> CombineTiling:
     return CombineTiling(split=int(plan.split_factor))
 
 
-def _check_tiling(spec, dense, split: bool = False) -> None:
+def _check_tiling(spec, dense, split: bool = False, shared: bool = False) -> None:
     if isinstance(spec, MLASpec) != isinstance(dense, DenseMLA):
         raise NotDenseAttention("the spec and the dense plan are not of the same operator family (GQA vs MLA)")
     if spec.kind not in BUILT_KINDS:
@@ -158,8 +158,10 @@ def _check_tiling(spec, dense, split: bool = False) -> None:
     if dense.query_rows < spec.group:
         raise UnsupportedTiling(f"a block's query tile holds {dense.query_rows} rows but the head group needs "
                                 f"{spec.group}; re-tile with at least {spec.group} query rows")
-    if getattr(spec, "shared_input", None) is not None:
-        raise UnsupportedTiling("no kernel reads shared pages yet")
+    if (getattr(spec, "shared_input", None) is not None) != shared:
+        raise UnsupportedTiling("shared pages are read by a kernel of their own (shared_variants), and by no other")
+    if shared and dense.head_dim > 256:
+        raise UnsupportedTiling(f"the kernel over shared pages has heads of at most 256 ({dense.head_dim})")
     if dense.head_dim % 32 or not (dense.head_dim % 128 == 0 or dense.head_dim == 64):
         raise UnsupportedTiling(f"head_dim {dense.head_dim} is not 64 or a multiple of 128")
 
@@ -221,6 +223,50 @@ def _plan(spec, dense, role, params, operands, split=None) -> KernelPlan:
     return KernelPlan(template="attn_decode", role=role, family="attention", dtype=dense.dtype, extra=extra,
                       problem=_paged_problem(spec, dense), tiling=tiling, params=params,
                       operands=operands, split_factor=split, dyn_dims=dyn, n_threads=dense.n_threads, label=label)
+
+
+# ----------------------------------------------------------------------------- decode over shared pages
+def shared_ranges(spec: PagingSpec) -> list:
+    """Launch-time numbers of ranges that the shared keys and a request's own keys are cut into: two workgroups on every compute
+    unit, ranges of four steps or more."""
+    from ...core.target import current_target
+
+    resident = 2 * current_target().arch.compute_units
+    b = spec.batch_dim
+    prefix = (f"max(1, min(ceildiv({spec.shared_dim} * {spec.page_size}, {4 * KV_STEP}), "
+              f"{resident} // ({spec.num_kv_heads} * max(1, ceildiv({b} * {spec.group}, 128)))))")
+    own = (f"max(1, min(ceildiv({spec.index_dim} * {spec.page_size}, {4 * KV_STEP} * max(1, {b})), "
+           f"{resident} // max(1, {b} * {spec.num_kv_heads * -(-spec.group // 16)})))")
+    return [("prefix_ranges", prefix), ("own_ranges", own)]
+
+
+def _shared_plan(spec: PagingSpec, dense: DenseAttention) -> KernelPlan:
+    """Parameter order: query, caches, shared pages, indptr, indices, [last page len], scale, out, lse."""
+    d, b, h = dense.head_dim, spec.batch_dim, spec.num_qo_heads
+    params, operands = _paged_params(spec, dense)
+    at = next(i for i, p in enumerate(params) if p.name == operands["INDPTR"])
+    shared = ParamSpec(f"PlaceHolder_{spec.shared_input}", "int32", (spec.shared_dim,), "input")
+    params[at] = dataclasses.replace(params[at], shape=(f"{b} + 1",))
+    params.insert(at, shared)
+    operands["SHARED"] = shared.name
+    outs, out_ops = _paged_outputs(spec, dense)
+    items = f"{b} * (prefix_ranges + own_ranges)"
+    for role, extents in (("PM", (items, h)), ("PL", (items, h)), ("PO", (items, h, d))):
+        names = [f"Partial_{role}_split", f"Partial_{role}_combine"]
+        params += [ParamSpec(names[0], "float32", extents, "scratch"), ParamSpec(names[1], "float32", extents, "scratch", alias=names[0])]
+        operands[role], operands[f"{role}_COMBINE"] = names
+    problem = _paged_problem(spec, dense)
+    problem["dim_names"] = {"batch": b, "num_pages": spec.pages_dim, "n_idx": spec.index_dim, "n_shared": spec.shared_dim}
+    return KernelPlan(template="attn_shared", role="main", family="attention", dtype=dense.dtype,
+                      extra={"derived_dims": shared_ranges(spec)}, problem=problem, tiling={}, params=params + outs,
+                      operands={**operands, **out_ops}, split_factor=None, dyn_dims=tuple(problem["dim_names"].values()), n_threads=256,
+                      label=f"shared pages kv={KV_STEP} q=128 thr=256")
+
+
+def shared_variants(plan: KernelPlan, spec) -> list:
+    dense = read_dense_attention(plan)
+    _check_tiling(spec, dense, shared=True)
+    return [_shared_plan(spec, dense)]
 
 
 MAX_CHUNK_PAGES = 64      # an item's page ids live in one register per lane of a wave
@@ -446,6 +492,8 @@ def apply_paging(plan: KernelPlan, spec, tok: int = 2, stages: int = 2, ksplit: 
         outs, out_ops = _mla_outputs(spec, dense)
         return _mla_plan(spec, dense, "main", params + outs, {**operands, **out_ops}, tok=tok, duo=duo)
     dense = read_dense_attention(plan)
+    if spec.shared_input is not None:
+        return shared_variants(plan, spec)[0]
     _check_tiling(spec, dense)
     if spec.kind in CAUSAL_KINDS:
         return _prefill_plan(spec, dense)
@@ -517,7 +565,7 @@ def can_page(plan, spec) -> bool:
 
     try:
         spec.validate()
-        _check_tiling(spec, read_dense(plan, spec))
+        _check_tiling(spec, read_dense(plan, spec), shared=getattr(spec, "shared_input", None) is not None)
     except PagingRefusal:
         return False
     return True

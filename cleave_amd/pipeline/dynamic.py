@@ -53,8 +53,10 @@ def _layer_variants(spec):
     the MLA prefill layer have several kernels per tiling and all of them go to the measurement."""
     from ..dynamic.paging import CAUSAL_KINDS, MLA_PAGED_PREFILL_CAUSAL, apply_paging
     from ..dynamic.paging import MLASpec
-    from ..dynamic.paging.apply import mla_decode_variants, mla_prefill_variants, prefill_variants
+    from ..dynamic.paging.apply import mla_decode_variants, mla_prefill_variants, prefill_variants, shared_variants
 
+    if getattr(spec, "shared_input", None) is not None:
+        return lambda tiled: shared_variants(tiled, spec)
     if spec.kind in CAUSAL_KINDS:
         return lambda tiled: prefill_variants(tiled, spec)
     if spec.kind == MLA_PAGED_PREFILL_CAUSAL:
@@ -97,7 +99,7 @@ def schedule_paged(graphs, spec, config, *, split_graphs=(), filter_before_topk=
             for form, source in emitted:
                 keep(graph, "solo", tile, dense, source, rank, form.label)
 
-    factors = tuple(config.split_k) if spec.kind in SPLIT_KINDS else ()
+    factors = tuple(config.split_k) if spec.kind in SPLIT_KINDS and getattr(spec, "shared_input", None) is None else ()
     for single in [p for p in plans if p.split_factor is None]:
         for factor in factors:
             combine = CombineTiling(split=factor, split_step=1, cols=min(128, single.dense.head_dim), n_threads=256)
@@ -653,8 +655,9 @@ def compile_dynamic(fn, *, dtype=None, preset="default", superopt=None, schedule
     body = attention.dense_body()
 
     split = (program.split or None) if split is None else split
-    if split and spec.kind not in SPLIT_KINDS:
-        search.note("split", f"split-KV is not built for the {spec.kind!r} layer; searching without it")
+    cuts_itself = getattr(spec, "shared_input", None) is not None          # (the kernel over shared pages, into ranges of its own)
+    if split and (spec.kind not in SPLIT_KINDS or cuts_itself):
+        search.note("split", f"split-KV is not built for the {spec.kind!r} layer{' over shared pages' * cuts_itself}; searching without it")
         split = False
     so, sc, ev = resolve_configs(body, preset=preset, superopt=superopt, schedule=schedule, eval=eval, split=split)
     if split is False:
