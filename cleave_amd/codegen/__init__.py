@@ -547,23 +547,25 @@ class HipCodeGen:
         unit.define("CL_ROWS", rows)
         unit.define("CL_WAVES", waves)
         unit.define("CL_PREFETCH", int(t.get("PREFETCH", 1)))
-        chunk_pages = bool(t.get("CHUNK_PAGES", 0)) and paged and (plan.split_factor or 1) > 1
+        items = paged and bool(p.get("window")) and bool(t.get("CHUNK_PAGES", 0)) and (plan.split_factor or 1) > 1
+        chunk_pages = not items and bool(t.get("CHUNK_PAGES", 0)) and paged and (plan.split_factor or 1) > 1
+        if items:
+            unit.define("CL_ITEMS", 1)
+            unit.define("CL_ITEM_RANGES", "ranges")
         unit.define("CL_CHUNK_PAGES", chunk_pages)
         if int(t.get("LOCKSTEP", 0)):
-            if not chunk_pages:
+            if not chunk_pages and not items:
                 raise CodegenError("LOCKSTEP (a barrier per step between the waves of a workgroup) exists for chunked items only")
             unit.define("CL_LOCKSTEP", 1)
         skew = int(t.get("SKEW", 0))
         if skew:
             # the rotation of units over the XCDs assumes that launch index % 8 is blockIdx.x % 8
             per_x = (p["kv_heads"] if paged else p["units"]) * (-(-rows // 16))
-            if (plan.split_factor or 1) % 2 or chunk_pages or per_x % 8 or not 0 < skew <= 500 or not partial:
+            if (plan.split_factor or 1) % 2 or chunk_pages or items or per_x % 8 or not 0 < skew <= 500 or not partial:
                 raise CodegenError("SKEW (split ranges skewed between even and odd XCDs, in thousandths of a pair's steps, "
                                    "1..500) needs an even split count, a grid of whole groups of eight unit tiles and no chunked items")
             unit.define("CL_SKEW", skew)
         if p.get("window"):
-            if chunk_pages:
-                raise CodegenError("a window has no chunked items")
             unit.define("CL_WINDOW", p["window"])
             unit.define("CL_SINKS", p["sinks"])
         unit.define("CL_PAGED", paged)
@@ -584,17 +586,20 @@ class HipCodeGen:
         if partial:
             from ..schedule.policy import attn_lds_bytes
 
-            if chunk_pages:
-                items = f"ceildiv({p['dim_names']['n_idx']}, chunk_pages) + {batch_name}"
-                grid = (items, 1, 1)
+            if items:
+                grid = (f"{batch_name} * ranges * {-(-p['kv_heads'] // waves) * row_tiles}", 1, 1)
+            elif chunk_pages:
+                grid = (f"ceildiv({p['dim_names']['n_idx']}, chunk_pages) + {batch_name}", 1, 1)
             else:
                 grid = (f"({units}) * {row_tiles}", splits, 1)
             # (a wave that shares its rows with no other stores straight from its accumulators: no LDS)
-            lds = 0 if waves == 1 or chunk_pages else attn_lds_bytes(waves, p["vdim"])
+            lds = 0 if waves == 1 or chunk_pages or items else attn_lds_bytes(waves, p["vdim"])
             unit.launch(ENTRY, grid, waves * 64, lds, self._partial_args)
         if combine:
             plain = f"ceildiv({grid_rows} * {p['vdim'] // 4}, 256)"
-            if chunk_pages:
+            if items:
+                self._launch_chunk_combine(unit, grid_rows, p["vdim"], f"{batch_name} * ranges")
+            elif chunk_pages:
                 self._launch_chunk_combine(unit, grid_rows, p["vdim"], f"ceildiv({p['dim_names']['n_idx']}, chunk_pages) + {batch_name}")
             elif paged:
                 unit.launch(self._combine_args[0], (plain, 1, 1), 256, 0, self._combine_args[1])
@@ -607,15 +612,15 @@ class HipCodeGen:
         d, group = p["head_dim"], p["group"]
         if plan.role != "main" or d % 64 or d > 256 or not (d == 64 or d % 128 == 0):
             raise CodegenError("attention over shared pages is one unsplit operator, of heads 64, 128 or 256 wide")
-        batch, ranges = p["dim_names"]["batch"], "(prefix_ranges + own_ranges)"
+        batch = p["dim_names"]["batch"]
         rows = f"({batch} * {p['q_heads']})"
-        plan = dataclasses.replace(plan, role="fused", split_factor=2)
+        plan = dataclasses.replace(plan, role="fused", split_factor=2, tiling={"CHUNK_PAGES": 1})       # (the sum reads the row pointers)
         self._attn_common(unit, plan, params, True, True, False, d, f"(batch * {p['q_heads']})", bool(p["emit_lse"]))
-        unit.define("CL_ITEM_RANGES", ranges)
-        by_name = self._by_name(params)
+        unit.define("CL_ITEM_RANGES", "prefix_ranges")
+        unit.define("CL_OWN_CHUNK", "own_chunk")
         names = [q.name for q in params if q.role in ("input", "scalar")] + [op[r] for r in ("PM", "PL", "PO")]
-        unit.define("CL_PARTIAL_ARGS", ", ".join([by_name[n].name for n in names] + list(p["dim_names"]) + [n for n, _ in plan.extra["derived_dims"]]))
-        for k, v in (("CL_PREFIX", 1), ("CL_OWN_PART", 1), ("CL_RAGGED", 0), ("CL_HEAD_DIM", d), ("CL_KV_HEADS", p["kv_heads"]),
+        unit.define("CL_PARTIAL_ARGS", ", ".join(names + list(p["dim_names"]) + [n for n, _ in plan.extra["derived_dims"]]))
+        for k, v in (("CL_PREFIX", 1), ("CL_OWN_PART", 1), ("CL_ITEMS", 1), ("CL_RAGGED", 0), ("CL_HEAD_DIM", d), ("CL_KV_HEADS", p["kv_heads"]),
                      ("CL_Q_HEADS", p["q_heads"]), ("CL_ROWS", group), ("CL_WAVES", 4), ("CL_PREFETCH", 1), ("CL_PAGED", 1),
                      ("CL_PAGE_SIZE", p["page_size"])):
             unit.define(k, v)
@@ -624,9 +629,10 @@ class HipCodeGen:
                 unit.define(f"CL_ARG_{role}", op[role])
         unit.templates += ["attn_tile.hip", "attn_prefill_lds.hip", "attn_decode.hip", "attn_shared.hip", "attn_combine.hip"]
         prefix = f"ceildiv({p['kv_heads']} * prefix_ranges, 8) * 8 * ceildiv({batch} * {group}, 128)"
-        own = f"{batch} * {p['kv_heads'] * -(-group // 16)} * own_ranges"
+        items = f"(ceildiv({p['dim_names']['n_idx']}, own_chunk) + {batch})"
+        own = f"{items} * {-(-p['kv_heads'] // 4) * -(-group // 16)}"
         unit.launch(ENTRY, (f"{prefix} + {own}", 1, 1), 256, 0, self._partial_args)
-        self._launch_chunk_combine(unit, rows, d, f"{batch} * {ranges}")
+        self._launch_chunk_combine(unit, rows, d, f"{batch} * prefix_ranges + {items}")
 
     def _emit_attn_dense_prefill(self, unit, plan, params, partial, combine):
         """The LDS-shared prefill kernel over the dense attention family's operands: every unit

@@ -4,12 +4,12 @@
 #ifndef CL_CHUNK_PAGES
 #define CL_CHUNK_PAGES 0
 #endif
-// CL_ITEM_RANGES: items are not cut from a page table; every request has that many (a run-time expression), one behind the other
-#ifndef CL_ITEM_RANGES
-#define CL_ITEM_RANGES 0
-#define CB_FIXED_ITEMS 0
-#else
+// CL_ITEM_RANGES: a run-time number of items that every request has first, one request's behind the other's.  With CL_OWN_CHUNK, the run-time
+// number of table entries of an item, items cut from the page table follow behind all of them.
+#ifdef CL_ITEM_RANGES
 #define CB_FIXED_ITEMS 1
+#else
+#define CB_FIXED_ITEMS 0
 #endif
 #ifndef CL_PO_ELEM
 #define CL_PO_ELEM 0
@@ -95,14 +95,26 @@ CL_COMBINE_NAME(CL_COMBINE_PARAMS) {
   auto add_up = [&](auto each, auto step, const i64 row, const int d, const int from, const int ahead) __attribute__((always_inline)) {
     constexpr int EACH = decltype(each)::value, STEP = decltype(step)::value;
     const int req = (int)(row / CL_Q_HEADS), qh = (int)(row % CL_Q_HEADS);
-#if CB_FIXED_ITEMS
-    const int count = CL_ITEM_RANGES, first = req * count;
+#if CB_FIXED_ITEMS && !defined(CL_OWN_CHUNK)
+    const int count = CL_ITEM_RANGES;
+    auto item_of = [&](const int it) { return (i64)req * count + it; };
 #else
+#ifdef CL_OWN_CHUNK
+    const int chunk_pages = CL_OWN_CHUNK;
+#endif
     int p0 = CL_CARG_INDPTR[req], p1 = CL_CARG_INDPTR[req + 1];
     p0 = p0 < 0 ? 0 : (p0 > n_idx ? n_idx : p0);
     p1 = p1 < 0 ? 0 : (p1 > n_idx ? n_idx : p1);
     const int first = req + p0 / chunk_pages;
-    const int count = p1 > p0 ? (p1 - 1) / chunk_pages - p0 / chunk_pages + 1 : 0;
+    int count = p1 > p0 ? (p1 - 1) / chunk_pages - p0 / chunk_pages + 1 : 0;
+#if CB_FIXED_ITEMS
+    count += CL_ITEM_RANGES;
+    auto item_of = [&](const int it) {
+      return it < CL_ITEM_RANGES ? (i64)req * CL_ITEM_RANGES + it : (i64)batch * CL_ITEM_RANGES + first + (it - CL_ITEM_RANGES);
+    };
+#else
+    auto item_of = [&](const int it) { return (i64)(first + it); };
+#endif
 #endif
     auto round = [&](auto whole, const int s) __attribute__((always_inline)) {
       constexpr int WHOLE = decltype(whole)::value;
@@ -111,7 +123,7 @@ CL_COMBINE_NAME(CL_COMBINE_PARAMS) {
 #pragma unroll
       for (int u = 0; u < EACH; ++u) {
         const int it = WHOLE || s + u * STEP < count ? s + u * STEP : count - 1;
-        const i64 prow = (i64)(first + it) * CL_Q_HEADS + qh;
+        const i64 prow = item_of(it) * CL_Q_HEADS + qh;
         pm[u] = CL_CARG_PM[prow];
         pl[u] = CL_CARG_PL[prow];
         po[u] = *reinterpret_cast<const f32x4*>(CL_CARG_PO + prow * CL_VDIM + d);

@@ -42,20 +42,30 @@
 //                s + skip behind it), so that splits share out what is seen; the ragged edges are masked.
 
 //   CL_OWN_PART  paged: not a kernel but the device function att_own_part(arguments, block) of attn_shared.hip: the requests' own keys
-//                behind pages that they share, cut into `own_ranges` (a run-time argument) parts whose partials lie behind those
-//                of the shared keys
+//                behind pages that they share, cut into items of `own_chunk` (a run-time argument) table entries whose partials
+//                lie behind those of the shared keys
+//   CL_ITEMS     what a window's or the own keys' split work is cut into (1; with CL_OWN_PART the latter): items of steps, one wave per
+//                kv head, CL_WAVES of them a workgroup; a window's are `ranges` (a run-time argument) equal parts of what each
+//                request sees.  The cache rows of an item's tokens are worked out once, into LDS: unseen tokens of its ragged
+//                steps repeat a seen one there.
 
 #define ATT_RAISE_BY 8.0f
 #ifndef CL_OWN_PART
 #define CL_OWN_PART 0
 #endif
-#if CL_OWN_PART
-#define ATT_SPLITS own_ranges
-#define ATT_PROW(split, orow) ((((orow) / CL_Q_HEADS) * (prefix_ranges + own_ranges) + prefix_ranges + (split)) * CL_Q_HEADS + (orow) % CL_Q_HEADS)
-#else
-#define ATT_SPLITS CL_SPLITS
-#define ATT_PROW(split, orow) ((i64)(split) * CL_TOTAL_ROWS + (orow))
+#ifndef CL_ITEMS
+#define CL_ITEMS 0
 #endif
+#if CL_OWN_PART && !CL_ITEMS
+#error "own keys come in items"
+#endif
+#if CL_OWN_PART
+#define ATT_SHARED_RANGES prefix_ranges
+#else
+#define ATT_SHARED_RANGES 0
+#endif
+#define ATT_BY_ITEM (CL_CHUNK_PAGES || CL_ITEMS)       // one wave per kv head, its partials by item
+#define ATT_LDS_ROWS ((CL_CHUNK_PAGES && CL_PAGE_SIZE == 1) || CL_ITEMS)
 #ifndef CL_WINDOW
 #define CL_WINDOW 0
 #endif
@@ -71,7 +81,7 @@
 #ifndef CL_LOCKSTEP
 #define CL_LOCKSTEP 0
 #endif
-#if CL_LOCKSTEP && !CL_CHUNK_PAGES
+#if CL_LOCKSTEP && !ATT_BY_ITEM
 #error "waves in step: chunked items only (every wave walks the same steps)"
 #endif
 #if CL_LOCKSTEP
@@ -85,7 +95,7 @@
 #define ATT_STEP 32
 #if CL_WINDOW
 #define ATT_SINK_STEPS ((CL_SINKS + ATT_STEP - 1) / ATT_STEP)
-#define ATT_T0(u, s) (((s) < ATT_SINK_STEPS ? (s) : (s) + (u).skip) * ATT_STEP)
+#define ATT_T0(u, s) (((s) + (u).first_step < ATT_SINK_STEPS ? (s) + (u).first_step : (s) + (u).first_step + (u).skip) * ATT_STEP)
 #define ATT_SEES(u, t) ((t) < (u).kv_len && ((t) >= (u).kv_len - CL_WINDOW || (t) < CL_SINKS))
 // (a key that is not seen is not read either: its page may be another's by now, and weight 0 times an infinite value is not 0)
 #define ATT_READ(u, t, last) (ATT_SEES(u, t) ? (t) : (last))
@@ -93,6 +103,11 @@
 #define ATT_READ(u, t, last) ((t) < (last) ? (t) : (last))
 #define ATT_T0(u, s) ((s) * ATT_STEP)
 #define ATT_SEES(u, t) ((t) < (u).kv_len)
+#endif
+#if ATT_LDS_ROWS
+#define ATT_LOAD_AT(u, s) ((s) * ATT_STEP)   // a step's rows in LDS
+#else
+#define ATT_LOAD_AT(u, s) ATT_T0(u, s)
 #endif
 #define ATT_KJ (CL_HEAD_DIM / 32)            // score MFMAs per 16 tokens
 #define ATT_VC ((CL_VDIM + 127) / 128)       // 128-wide value chunks
@@ -106,6 +121,7 @@ struct AttUnit {
   int kv_len;           // valid tokens
 #if CL_WINDOW
   int skip;             // 32-token steps between the sinks' last one and the window's first one
+  int first_step;       // of an item (0 where steps are numbered from the request's first)
 #endif
   int rows;             // real rows in this tile (1..16)
   const int* pages;     // paged: this request's slice of the page table
@@ -115,7 +131,14 @@ struct AttUnit {
   i64 out_row;          // flattened (unit, row) index of the tile's first row
 };
 
-#if CL_PAGED && CL_CHUNK_PAGES && CL_PAGE_SIZE == 1
+#if CL_ITEMS
+#define ATT_MAX_IDS 2048
+#if CL_OWN_PART
+#define att_ids reinterpret_cast<int*>(pl_tiles)      // (the shared keys' images: a workgroup of own keys has none)
+#else
+__shared__ __attribute__((aligned(16))) int att_ids[ATT_MAX_IDS];
+#endif
+#elif CL_PAGED && CL_CHUNK_PAGES && CL_PAGE_SIZE == 1
 // Token tables: the (clamped) ids of an item's tokens lie in LDS, read once by all waves, the last one repeated up to a whole step.
 // (A lane's registers hold 64 of them, two steps; a table load per token would sit in the same in-order queue as the rows.)
 #define ATT_MAX_IDS 2048
@@ -152,7 +175,7 @@ struct AttTile {               // one 32-token step's K and V, as loaded
 // Issue the loads of the step starting at token t0.  Tokens past kv_len are clamped onto the
 // last valid token (their scores are masked later), so no load leaves the tensor.
 CL_DEVICE void att_load(const AttUnit& u, int t0, int c, int g, AttTile& tile) {
-#if CL_PAGED && CL_CHUNK_PAGES && CL_PAGE_SIZE == 1
+#if ATT_LDS_ROWS
   typedef int att_i32x4 __attribute__((ext_vector_type(4)));
   const int id_k[2] = {att_ids[t0 + c], att_ids[t0 + 16 + c]};
   const att_i32x4 id_v[2] = {*reinterpret_cast<const att_i32x4*>(&att_ids[t0 + 4 * g]), *reinterpret_cast<const att_i32x4*>(&att_ids[t0 + 16 + 4 * g])};
@@ -197,11 +220,11 @@ CL_DEVICE void att_load(const AttUnit& u, int t0, int c, int g, AttTile& tile) {
 #endif
 }
 
-#if CL_CHUNK_PAGES
+#if CL_CHUNK_PAGES || (CL_ITEMS && CL_OWN_PART)
 // Work items in page-table order: a new item starts at every multiple of chunk_pages table
 // entries and at every request boundary, so item t = (chunk w) + (request b) for the one pair
 // with chunk w overlapping request b.  Request b owns items b + p0/C .. b + (p1-1)/C.
-static_assert(CL_PAGED && CL_ROWS <= 16 && CL_WAVES == CL_KV_HEADS, "chunked items: one wave per kv head");
+static_assert(CL_PAGED && (CL_ITEMS || (CL_ROWS <= 16 && CL_WAVES == CL_KV_HEADS)), "chunked items: one wave per kv head");
 CL_DEVICE int att_clamp_ptr(int p, int n_idx) { return p < 0 ? 0 : (p > n_idx ? n_idx : p); }
 #endif
 
@@ -226,12 +249,16 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
 #if CL_CHUNK_PAGES
   const int split = 0, tile_id = 0;
   const int item = blockIdx.x;
-#elif CL_OWN_PART
-  // (as a grid of (units, ranges) is laid out)
-  const int split = block / (batch * CL_KV_HEADS * ATT_ROW_TILES);
-  const int unit_tile = block % (batch * CL_KV_HEADS * ATT_ROW_TILES);
-  const int tile_id = unit_tile % ATT_ROW_TILES;
-  const int unit = unit_tile / ATT_ROW_TILES;
+#elif CL_ITEMS
+  // an item's workgroups (CL_WAVES kv heads and one 16-row tile each) next to each other: they read neighbouring pieces of the same rows
+#if !CL_OWN_PART
+  const int block = blockIdx.x;
+#endif
+  constexpr int head_groups = (CL_KV_HEADS + CL_WAVES - 1) / CL_WAVES;
+  const int split = 0, tile_id = block / head_groups % ATT_ROW_TILES;
+  const int item = block / (head_groups * ATT_ROW_TILES);
+  const int my_head = block % head_groups * CL_WAVES + wave;
+  const int head = my_head < CL_KV_HEADS ? my_head : CL_KV_HEADS - 1;      // (a wave past the last head keeps step and stores nothing)
 #else
   const int split = blockIdx.y;
 #if CL_SKEW
@@ -292,12 +319,46 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
   u.out_row = (i64)req * CL_Q_HEADS + (i64)head * CL_ROWS;
   u.q = CL_ARG_Q + u.out_row * CL_HEAD_DIM;
   const float scale2 = sm_scale * 1.4426950408889634f;
+#elif CL_ITEMS
+#if CL_OWN_PART
+  const ClRequest found = cl_find_request(CL_ARG_INDPTR, batch, n_idx, own_chunk, 1, item, lane);
+  const int req = found.req, p0 = found.p0, p1 = found.p1;
+  const int chunk = item - req;
+  const int lo = p0 > chunk * own_chunk ? p0 : chunk * own_chunk;
+  const int hi = p1 < (chunk + 1) * own_chunk ? p1 : (chunk + 1) * own_chunk;
+  if (hi <= lo) return;                               // an index no (chunk, request) pair maps to
+#else
+  const int req = item / ranges;
+  const int lo = cl_clamp_ptr(CL_ARG_INDPTR[req], n_idx), p1 = cl_clamp_ptr(CL_ARG_INDPTR[req + 1], n_idx);
+  const int hi = p1 > lo ? p1 : lo;
+#endif
+  u.pages = CL_ARG_INDICES + lo;
+  u.n_pages = hi - lo;
+  u.pool_pages = num_pages;
+  u.page_reg = 0;
+  {
+    int lastp = CL_PAGE_SIZE;
+#if CL_PAGE_SIZE > 1
+    if (hi == p1 && u.n_pages > 0) {
+      lastp = CL_ARG_LAST[req];
+      lastp = lastp > 0 ? (lastp < CL_PAGE_SIZE ? lastp : CL_PAGE_SIZE) : 0;
+    }
+#endif
+    u.kv_len = u.n_pages > 0 ? (u.n_pages - 1) * CL_PAGE_SIZE + lastp : 0;
+  }
+  u.k_stride = (i64)CL_KV_HEADS * CL_HEAD_DIM;
+  u.v_stride = (i64)CL_KV_HEADS * CL_VDIM;
+  u.k = CL_ARG_K + (i64)head * CL_HEAD_DIM;
+  u.v = CL_ARG_V + (i64)head * CL_VDIM;
+  u.out_row = (i64)req * CL_Q_HEADS + (i64)head * CL_ROWS + 16 * tile_id;
+  u.q = CL_ARG_Q + u.out_row * CL_HEAD_DIM;
+  const float scale2 = sm_scale * 1.4426950408889634f;
 #elif CL_PAGED
   // unit = request * kv_heads + kv head.  The request's length follows the page-granular
   // CSR: every page but the last is full, the last holds kv_last_page_len tokens, and the
   // sum is clamped to the pages the request owns.
   const int req = unit / CL_KV_HEADS, head = unit % CL_KV_HEADS;
-#if CL_WINDOW || CL_OWN_PART
+#if CL_WINDOW
   const int p0 = cl_clamp_ptr(CL_ARG_INDPTR[req], n_idx), p1 = cl_clamp_ptr(CL_ARG_INDPTR[req + 1], n_idx);
 #else
   const int p0 = CL_ARG_INDPTR[req], p1 = CL_ARG_INDPTR[req + 1];
@@ -346,13 +407,33 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
 
   // This split's steps: ceil(n_steps / SPLITS) each; a trailing split may own none.
 #if CL_WINDOW
+  u.first_step = 0;
   u.skip = (u.kv_len > CL_WINDOW ? u.kv_len - CL_WINDOW : 0) / ATT_STEP - ATT_SINK_STEPS;
   u.skip = u.skip > 0 ? u.skip : 0;
   const int n_steps = (u.kv_len + ATT_STEP - 1) / ATT_STEP - u.skip;
 #else
   const int n_steps = (u.kv_len + ATT_STEP - 1) / ATT_STEP;
 #endif
-#if CL_CHUNK_PAGES
+#if CL_ITEMS
+#if CL_WINDOW
+  const int per_range = (n_steps + ranges - 1) / ranges;
+  u.first_step = item % ranges * per_range;
+  int left = n_steps - u.first_step;
+  left = left < per_range ? left : per_range;
+  const int step_begin = 0, step_end = left > 0 ? left : 0;
+#else
+  const int step_begin = 0, step_end = n_steps;
+#endif
+  for (int i = threadIdx.x; i < step_end * ATT_STEP; i += CL_WAVES * 64) {
+    int t = ATT_T0(u, i / ATT_STEP) + i % ATT_STEP;
+    t = ATT_READ(u, t, u.kv_len - 1);
+    int pid = u.pages[t / CL_PAGE_SIZE];
+    pid = pid < num_pages - 1 ? pid : num_pages - 1;
+    att_ids[i] = (pid > 0 ? pid : 0) * CL_PAGE_SIZE + t % CL_PAGE_SIZE;
+  }
+  __syncthreads();
+  (void)split;
+#elif CL_CHUNK_PAGES
   const int step_begin = 0, step_end = n_steps;      // the item is the unit of work: no further cut
   (void)split;
 #elif CL_SKEW
@@ -373,7 +454,7 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
     step_end = (split & 1) == 0 ? lo + first : hi;
   }
 #else
-  const int per_split = (n_steps + ATT_SPLITS - 1) / ATT_SPLITS;
+  const int per_split = (n_steps + CL_SPLITS - 1) / CL_SPLITS;
   const int step_begin = split * per_split;
   int step_end = step_begin + per_split;
   step_end = step_end < n_steps ? step_end : n_steps;
@@ -404,7 +485,7 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
   // steps n+1 .. n+CL_PREFETCH are in flight.  The ring position is a compile-time constant of
   // the unrolled inner loop, so every tile stays in registers.
   AttTile ring[CL_PREFETCH + 1];
-#if CL_CHUNK_PAGES
+#if ATT_BY_ITEM
 #define ATT_WSTRIDE 1                 // every wave walks all steps of the item for its own head
   const int step0 = step_begin;
 #else
@@ -437,7 +518,7 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
 #define ATT_ONE_STEP(R, STEP, LOAD)                                                                 \
     {                                                                                               \
       ATT_LOCKSTEP()                                                                                \
-      if (LOAD) att_load(u, ATT_T0(u, (STEP) + CL_PREFETCH * ATT_WSTRIDE), c, g, ring[((R) + CL_PREFETCH) % (CL_PREFETCH + 1)]); \
+      if (LOAD) att_load(u, ATT_LOAD_AT(u, (STEP) + CL_PREFETCH * ATT_WSTRIDE), c, g, ring[((R) + CL_PREFETCH) % (CL_PREFETCH + 1)]); \
       const AttTile& cur = ring[R];                                                                 \
       const int t0 = ATT_T0(u, STEP);                                                               \
                                                                                                     \
@@ -495,7 +576,7 @@ _Pragma("unroll")                                                               
   if (step0 < step_end) {
 #pragma unroll
     for (int i = 0; i < CL_PREFETCH; ++i)
-      if (step0 + i * ATT_WSTRIDE < step_end) att_load(u, ATT_T0(u, step0 + i * ATT_WSTRIDE), c, g, ring[i]);
+      if (step0 + i * ATT_WSTRIDE < step_end) att_load(u, ATT_LOAD_AT(u, step0 + i * ATT_WSTRIDE), c, g, ring[i]);
     int base = step0;
     for (; base + 2 * CL_PREFETCH * ATT_WSTRIDE < step_end; base += (CL_PREFETCH + 1) * ATT_WSTRIDE) {
 #pragma unroll
@@ -510,17 +591,13 @@ _Pragma("unroll")                                                               
 
   l_run += lane_xor(l_run, lane, 16);
   l_run += lane_xor(l_run, lane, 32);
-#if CL_WAVES > 1 && !CL_CHUNK_PAGES
+#if CL_WAVES > 1 && !ATT_BY_ITEM
   // ---- the workgroup's waves merged into its first one through LDS: every other wave leaves its
   // reference points, weight sums and accumulators as they lie in its registers (one 16-byte piece
   // per lane and accumulator: whole 1 KiB rows), and the first wave folds them into its own by the
   // max-rescale rule: one LDS round trip for all of them --------------------------------------
   {
-#if CL_OWN_PART
-    float* att_lds = reinterpret_cast<float*>(pl_tiles);                      // (the shared keys' images: this workgroup has none)
-#else
     extern __shared__ float att_lds[];
-#endif
     f32x4* sh_o = reinterpret_cast<f32x4*>(att_lds);                          // [WAVES - 1][8 ATT_VC][64]
     float* sh_m = att_lds + (CL_WAVES - 1) * 8 * ATT_VC * 64 * 4;              // [WAVES - 1][16]
     float* sh_l = sh_m + (CL_WAVES - 1) * 16;                                  // [WAVES - 1][16]
@@ -564,14 +641,22 @@ _Pragma("unroll")                                                               
   // ---- the rows leave straight from the accumulators of the wave that owns them (the first wave of
   // a workgroup; every wave of a chunked item, which owns one kv head): lane (c, g) holds, of row c,
   // the eight neighbours from 128 vc + 32 g + 8 r on for every r --------------------------------
+#if CL_ITEMS
+  if (my_head >= CL_KV_HEADS) return;
+#endif
   if (c < u.rows) {
     const i64 orow = u.out_row + c;
-#if CL_CHUNK_PAGES
+#if CL_ITEMS
+    // (items by number; of own keys, behind the shared keys' partials)
+    const i64 prow = ((i64)item + (CL_OWN_PART ? (i64)batch * ATT_SHARED_RANGES : 0)) * CL_Q_HEADS + (i64)head * CL_ROWS + 16 * tile_id + c;
+    float* dst = CL_ARG_PO + prow * CL_VDIM;
+    (void)orow;
+#elif CL_CHUNK_PAGES
     const i64 prow = (i64)item * CL_Q_HEADS + (i64)head * CL_ROWS + c;      // partials are (item, query head[, d])
     float* dst = CL_ARG_PO + prow * CL_VDIM;
     (void)orow;
 #elif CL_SPLITS > 1
-    const i64 prow = ATT_PROW(split, orow);
+    const i64 prow = (i64)split * CL_TOTAL_ROWS + orow;
     float* dst = CL_ARG_PO + prow * CL_VDIM;
 #else
     elem_t* dst = CL_ARG_OUT + orow * CL_VDIM;
@@ -583,7 +668,7 @@ _Pragma("unroll")                                                               
       for (int r = 0; r < 4; ++r) {
         const int d0 = 128 * vc + 32 * g + 8 * r;
         if (CL_VDIM % 128 != 0 && d0 >= CL_VDIM) continue;
-#if CL_SPLITS > 1 || CL_CHUNK_PAGES
+#if CL_SPLITS > 1 || ATT_BY_ITEM
         *reinterpret_cast<f32x4*>(dst + d0) = (f32x4){acc[vc][0][r], acc[vc][1][r], acc[vc][2][r], acc[vc][3][r]};
         *reinterpret_cast<f32x4*>(dst + d0 + 4) = (f32x4){acc[vc][4][r], acc[vc][5][r], acc[vc][6][r], acc[vc][7][r]};
 #else
@@ -594,7 +679,7 @@ _Pragma("unroll")                                                               
 #endif
       }
     if (g == 0) {
-#if CL_SPLITS > 1 || CL_CHUNK_PAGES
+#if CL_SPLITS > 1 || ATT_BY_ITEM
       CL_ARG_PM[prow] = m_run;
       CL_ARG_PL[prow] = l_run;
 #elif CL_EMIT_LSE

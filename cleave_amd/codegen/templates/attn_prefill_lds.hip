@@ -112,7 +112,7 @@
 #endif
 #if CL_PREFIX
 #define PL_TABLE CL_ARG_SHARED
-#define PL_PROW(split, m) ((((i64)(lo + (m)) / PL_GROUP) * (prefix_ranges + own_ranges) + (split)) * CL_Q_HEADS + head * PL_GROUP + (lo + (m)) % PL_GROUP)
+#define PL_PROW(split, m) ((((i64)(lo + (m)) / PL_GROUP) * prefix_ranges + (split)) * CL_Q_HEADS + head * PL_GROUP + (lo + (m)) % PL_GROUP)
 #define PL_PAGE(pos) ((pos) / CL_PAGE_SIZE)
 #define PL_ROW(page, pos) ((page) * CL_PAGE_SIZE + (pos) % CL_PAGE_SIZE)
 #else
@@ -144,13 +144,7 @@ static_assert(CL_HEAD_DIM % 64 == 0 && CL_HEAD_DIM <= 256 && CL_VDIM % 64 == 0 &
               "key and value widths in whole 64-feature panels");
 static_assert(PL_UNITS_PER < 16, "load counter range");
 
-#if CL_PREFIX
-// (the workgroups of the other part merge their waves here: 8 KiB and 128 bytes of each but the first per 128 value features)
-#define PL_MERGE (3 * ((CL_VDIM + 127) / 128 * 4096 + 64))
-__shared__ __attribute__((aligned(1024))) elem_t pl_tiles[PL_STAGES * PL_STAGE > PL_MERGE ? PL_STAGES * PL_STAGE : PL_MERGE];
-#else
 __shared__ __attribute__((aligned(1024))) elem_t pl_tiles[PL_STAGES * PL_STAGE];
-#endif
 #if !CL_RAGGED
 __shared__ __attribute__((aligned(256))) int pl_ids[2][4][64];   // table entries on their way in: [step parity][wave][lane]
 #endif

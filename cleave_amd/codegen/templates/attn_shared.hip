@@ -5,13 +5,13 @@
 //   shared keys  read once for the whole batch: the queries of all requests are the rows of one matrix product per kv head
 //                (pl_prefix_part, attn_prefill_lds.hip: 128 rows a workgroup, key tiles through LDS);
 //   own keys     read by their request alone (att_own_part, attn_decode.hip: registers, nothing through LDS on the way in);
-//   partials     of `prefix_ranges` ranges of the shared keys and `own_ranges` of a request's own, f32, request-major
-//                (request, range, query head[, d]), merged by attn_combine.hip.
+//   partials     of `prefix_ranges` ranges of the shared keys (request, range, query head[, d]) and, behind them, of items of
+//                `own_chunk` entries of the requests' own table (item, query head[, d]), f32, merged by attn_combine.hip.
 // Read by every request for itself, the shared keys would be `batch` times the traffic.
 //
 // One launch holds both kinds: the first part is bound by the matrix cores or L2, the second by HBM, and their workgroups run beside
 // each other.
-//   run-time: batch, num_pages, n_shared (shared pages), n_idx (own table length), prefix_ranges, own_ranges, sm_scale
+//   run-time: batch, num_pages, n_shared (shared pages), n_idx (own table length), prefix_ranges, own_chunk, sm_scale
 extern "C" __global__ void __launch_bounds__(256, 2)
 CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
   const int row_tiles = (batch * PL_GROUP + PL_ROWS - 1) / PL_ROWS;

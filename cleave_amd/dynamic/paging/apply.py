@@ -160,8 +160,9 @@ def _check_tiling(spec, dense, split: bool = False, shared: bool = False) -> Non
                                 f"{spec.group}; re-tile with at least {spec.group} query rows")
     if (getattr(spec, "shared_input", None) is not None) != shared:
         raise UnsupportedTiling("shared pages are read by a kernel of their own (shared_variants), and by no other")
-    if shared and dense.head_dim > 256:
-        raise UnsupportedTiling(f"the kernel over shared pages has heads of at most 256 ({dense.head_dim})")
+    if shared and (dense.head_dim > 256 or spec.page_size > MAX_CHUNK_TOKENS):
+        raise UnsupportedTiling(f"the kernel over shared pages has heads of at most 256 ({dense.head_dim}) and pages of at most "
+                                f"{MAX_CHUNK_TOKENS} tokens ({spec.page_size})")
     if dense.head_dim % 32 or not (dense.head_dim % 128 == 0 or dense.head_dim == 64):
         raise UnsupportedTiling(f"head_dim {dense.head_dim} is not 64 or a multiple of 128")
 
@@ -212,7 +213,12 @@ def _plan(spec, dense, role, params, operands, split=None) -> KernelPlan:
     label = f"kv={dense.kv_tile} q={dense.query_rows} thr={dense.n_threads}"
     tiling = {"WAVES": dense.waves, "PREFETCH": dense.prefetch}
     extra = {}
-    if dense.chunk_pages and split:
+    if dense.chunk_pages and split and spec.window is not None:
+        tiling.update(WAVES=min(spec.num_kv_heads, 8), CHUNK_PAGES=dense.chunk_pages)
+        if dense.lockstep and role != "combine":
+            tiling["LOCKSTEP"] = 1
+        extra["derived_dims"] = [("ranges", window_ranges_expr(spec, dense.chunk_pages))]
+    elif dense.chunk_pages and split:
         tiling.update(WAVES=spec.num_kv_heads, CHUNK_PAGES=dense.chunk_pages)
         if dense.lockstep and role != "combine":
             tiling["LOCKSTEP"] = 1
@@ -227,17 +233,19 @@ def _plan(spec, dense, role, params, operands, split=None) -> KernelPlan:
 
 # ----------------------------------------------------------------------------- decode over shared pages
 def shared_ranges(spec: PagingSpec) -> list:
-    """Launch-time numbers of ranges that the shared keys and a request's own keys are cut into: two workgroups on every compute
-    unit, ranges of four steps or more."""
+    """Launch-time cuts: the number of ranges of the shared keys, and the table entries of an item of the requests' own: two
+    workgroups on every compute unit, ranges and items of four steps or more."""
     from ...core.target import current_target
 
     resident = 2 * current_target().arch.compute_units
     b = spec.batch_dim
     prefix = (f"max(1, min(ceildiv({spec.shared_dim} * {spec.page_size}, {4 * KV_STEP}), "
               f"{resident} // ({spec.num_kv_heads} * max(1, ceildiv({b} * {spec.group}, 128)))))")
-    own = (f"max(1, min(ceildiv({spec.index_dim} * {spec.page_size}, {4 * KV_STEP} * max(1, {b})), "
-           f"{resident} // max(1, {b} * {spec.num_kv_heads * -(-spec.group // 16)})))")
-    return [("prefix_ranges", prefix), ("own_ranges", own)]
+    pieces = -(-spec.num_kv_heads // 4) * -(-spec.group // 16)                  # workgroups of an item
+    most = max(1, MAX_CHUNK_TOKENS // spec.page_size)
+    least = max(1, 4 * KV_STEP // spec.page_size)
+    own = f"max({min(least, most)}, min({most}, ceildiv({spec.index_dim} * {pieces}, {resident})))"
+    return [("prefix_ranges", prefix), ("own_chunk", own)]
 
 
 def _shared_plan(spec: PagingSpec, dense: DenseAttention) -> KernelPlan:
@@ -250,7 +258,7 @@ def _shared_plan(spec: PagingSpec, dense: DenseAttention) -> KernelPlan:
     params.insert(at, shared)
     operands["SHARED"] = shared.name
     outs, out_ops = _paged_outputs(spec, dense)
-    items = f"{b} * (prefix_ranges + own_ranges)"
+    items = f"{b} * prefix_ranges + ceildiv({spec.index_dim}, own_chunk) + {b}"
     for role, extents in (("PM", (items, h)), ("PL", (items, h)), ("PO", (items, h, d))):
         names = [f"Partial_{role}_split", f"Partial_{role}_combine"]
         params += [ParamSpec(names[0], "float32", extents, "scratch"), ParamSpec(names[1], "float32", extents, "scratch", alias=names[0])]
@@ -289,6 +297,18 @@ def chunk_pages_expr(spec, chunk_pages: int) -> str:
         return f"max(32, min({MAX_CHUNK_TOKENS}, ceildiv(ceildiv({spec.index_dim}, max(1, {cus} - {spec.batch_dim})), 32) * 32))"
     return (f"max(1, min({MAX_CHUNK_PAGES}, ceildiv({spec.index_dim}, "
             f"max(1, {cus} - {spec.batch_dim}))))")
+
+
+def window_ranges_expr(spec, ranges: int) -> str:
+    """The launch-time number of ranges that what a request sees of a window is cut into: the fixed value, or for -1 the one that gives
+    every compute unit an item; ranges of at most the 64 steps whose rows fit an item's LDS, and of two or more."""
+    from ...core.target import current_target
+
+    steps = -(-(spec.window + KV_STEP - 1) // KV_STEP) + -(-spec.sinks // KV_STEP)     # (a window begins and ends inside a step)
+    least = -(-steps // (MAX_CHUNK_TOKENS // KV_STEP))
+    if ranges > 0:
+        return str(max(least, ranges))
+    return f"max({least}, min({max(1, steps // 2)}, {current_target().arch.compute_units} // max(1, {spec.batch_dim})))"
 
 
 # ----------------------------------------------------------------------------- causal prefill
@@ -518,13 +538,14 @@ def build_split_decode(spec, dense: DenseAttention, split: int, comb: CombineTil
     # (python/cleave/dynamic/paging/tensor_maps.py:41-69)
     if dense.chunk_pages:
         if spec.window is not None:
-            raise UnsupportedTiling("items of a page table are cut from all of a request's pages: a window has the fixed split")
-        if dense.chunk_pages < -1 or dense.chunk_pages > max_chunk_pages(spec) or dense.query_rows > 16 \
+            if dense.chunk_pages < -1:
+                raise UnsupportedTiling("items of a window: a positive number of ranges, or -1 (chosen at launch)")
+        elif dense.chunk_pages < -1 or dense.chunk_pages > max_chunk_pages(spec) or dense.query_rows > 16 \
                 or spec.num_kv_heads > 16:
             raise UnsupportedTiling(f"chunked items need chunk_pages in 1..{max_chunk_pages(spec)} (or -1), one 16-row "
                                     "query tile and at most 16 kv heads")
         # one partial per work item: a new item at every chunk_pages table entries and every request
-        items = f"ceildiv({spec.index_dim}, chunk_pages) + {b}"
+        items = f"ceildiv({spec.index_dim}, chunk_pages) + {b}" if spec.window is None else f"{b} * ranges"
         bufs = [("PM", (items, h)), ("PL", (items, h)), ("PO", (items, h, d))]
     else:
         bufs = [("PM", (split, b, h)), ("PL", (split, b, h)), ("PO", (split, b, h, d))]

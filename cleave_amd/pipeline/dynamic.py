@@ -116,7 +116,12 @@ def schedule_paged(graphs, spec, config, *, split_graphs=(), filter_before_topk=
                 # split / these: 64 requests, 68237 tokens 66 / 41.6, 40 of up to 4000 91 / 66, 23 of 2682 40 / 28.8, 18 of 1056 16.2 / 14.9;
                 # behind the fixed split for four requests and fewer, 3 of 2882 11.5 / 12.9, which keep it by the calibrated rule, and the single
                 # kernel for short ones, 63 of 50 8.1 / 10.5)
-                if getattr(spec, "window", None) is None and (getattr(spec, "page_size", 1) == 1 or spec.page_size >= 16) and single.dense.query_rows <= 16 and factor == max(factors):
+                if getattr(spec, "window", None) is not None:
+                    # (a window: equal parts of what is seen, as many as give every compute unit one, instead of a number of the search's)
+                    if factor == max(factors):
+                        forms.append(dataclasses.replace(single.dense, chunk_pages=-1, lockstep=True, waves=min(spec.num_kv_heads, 8),
+                                                         n_threads=min(spec.num_kv_heads, 8) * 64))
+                elif (getattr(spec, "page_size", 1) == 1 or spec.page_size >= 16) and single.dense.query_rows <= 16 and factor == max(factors):
                     forms.append(dataclasses.replace(single.dense, chunk_pages=-1, lockstep=True, waves=spec.num_kv_heads,
                                                      n_threads=spec.num_kv_heads * 64))
             for d in forms:

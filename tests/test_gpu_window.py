@@ -27,10 +27,11 @@ def compiled(source):
 
 
 # ------------------------------------------------------------------------------------------------ decode
-def decode_kernel(page, window, sinks, hq=8, hkv=2, d=128, dtype="float16", waves=4, split=None, prefetch=1, skew=0):
+def decode_kernel(page, window, sinks, hq=8, hkv=2, d=128, dtype="float16", waves=4, split=None, prefetch=1, skew=0, ranges=0, lockstep=True):
     spec = PagingSpec(hq, hkv, kind=PAGED_DECODE_SLAB if page > 1 else PAGED_DECODE, page_size=page, window=window, sinks=sinks)
     spec.validate()
-    dense = DenseAttention(-(-hq // hkv // 16) * 16, 32, d, waves * 64, dtype, dtype, waves=waves, prefetch=prefetch, skew=skew)
+    dense = DenseAttention(-(-hq // hkv // 16) * 16, 32, d, waves * 64, dtype, dtype, waves=waves, prefetch=prefetch, skew=skew,
+                           chunk_pages=ranges, lockstep=lockstep and ranges != 0)
     if split:
         return compiled(HipCodeGen().gen(build_split_decode(spec, dense, split, CombineTiling(split=split, cols=min(128, d)))))
     params, ops = _paged_params(spec, dense)
@@ -73,6 +74,34 @@ def test_decode(page, split, window, sinks):
     check_decode(decode_kernel(page, window, sinks, split=split), decode_args(LENS, page), LENS, page, window, sinks)
 
 
+@pytest.mark.parametrize("page", [1, 16, 64])
+@pytest.mark.parametrize("ranges", [-1, 1, 5])
+@pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (31, 0), (32, 4), (33, 32), (64, 33), (100, 100), (97, 1), (2000, 4), (40, 400)])
+def test_decode_by_items(page, ranges, window, sinks):
+    """What is seen in equal parts by workgroups of one wave per kv head; more parts than steps leave some empty."""
+    print(f"window decode by items page={page} ranges={ranges} window={window} sinks={sinks}", flush=True)
+    check_decode(decode_kernel(page, window, sinks, split=2, ranges=ranges), decode_args(LENS, page), LENS, page, window, sinks)
+
+
+@pytest.mark.parametrize("kw", [dict(hq=24, hkv=12), dict(hq=9, hkv=3), dict(hq=40, hkv=2), dict(d=64), dict(d=256, hq=6), dict(hq=32, hkv=8, dtype="bfloat16"),
+                                dict(hq=32, hkv=8, lockstep=False), dict(prefetch=2)], ids=lambda kw: "_".join(f"{k}{v}" for k, v in kw.items()))
+def test_decode_by_items_forms(kw):
+    lens = [70, 3, 900, 129, 0]
+    shape = {k: v for k, v in kw.items() if k in ("hq", "hkv", "d")}
+    for page in (1, 64):
+        print(f"window decode by items {kw} page={page}", flush=True)
+        args = decode_args(lens, page, dtype=getattr(torch, kw.get("dtype", "float16")), **shape)
+        check_decode(decode_kernel(page, 130, 5, split=2, ranges=-1, **kw), args, lens, page, 130, 5)
+
+
+def test_decode_window_of_many_items():
+    """A window of more rows than an item's LDS holds."""
+    lens, window, sinks = [9000, 5000, 4], 4500, 700
+    args = decode_args(lens, 16)
+    print("window decode by items of a long window", flush=True)
+    check_decode(decode_kernel(16, window, sinks, split=2, ranges=1), args, lens, 16, window, sinks)
+
+
 @pytest.mark.parametrize("kw", [dict(waves=1), dict(waves=2, prefetch=2), dict(waves=8, split=2), dict(waves=1, split=4, hkv=8, hq=32, skew=30),
                                 dict(d=64), dict(d=256, hq=6, waves=2), dict(dtype="bfloat16", hq=16, hkv=2, split=3), dict(hq=40, hkv=2)],
                          ids=lambda kw: "_".join(f"{k}{v}" for k, v in kw.items()))
@@ -86,9 +115,9 @@ def test_decode_forms(kw):
 
 
 @pytest.mark.parametrize("page", [1, 64])
-@pytest.mark.parametrize("split", [None, 8])
+@pytest.mark.parametrize("split,ranges", [(None, 0), (8, 0), (2, -1), (2, 3)])
 @pytest.mark.parametrize("value", [math.inf, math.nan])
-def test_decode_never_reads_what_is_not_seen(page, split, value):
+def test_decode_never_reads_what_is_not_seen(page, split, ranges, value):
     """Keys and values outside window and sinks are undefined: pages that a server has handed on to other requests."""
     lens, window, sinks = [700, 90, 333], 100, 3
     args = decode_args(lens, page)
@@ -99,8 +128,8 @@ def test_decode_never_reads_what_is_not_seen(page, split, value):
         hidden = hidden[(hidden < n - window) & (hidden >= sinks)]
         for cache in args[1:3]:
             cache[page_of[hidden], slot[hidden]] = value
-    print(f"window decode hidden={value} page={page} split={split}", flush=True)
-    out, lse = decode_kernel(page, window, sinks, split=split)(*args)
+    print(f"window decode hidden={value} page={page} split={split} ranges={ranges}", flush=True)
+    out, lse = decode_kernel(page, window, sinks, split=split, ranges=ranges)(*args)
     same(out, want[0], want[2], "out")
     same(lse, want[1], want[3], "lse")
 

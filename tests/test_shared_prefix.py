@@ -107,12 +107,13 @@ def test_launch_time_cuts(hq, hkv, page):
                 for name, expr in manifest["derived_dims"]:
                     dims[name] = eval_extent(expr, dims)
                     postfix(expr, {n: i for i, n in enumerate(dims)})
-                assert dims["prefix_ranges"] >= 1 and dims["own_ranges"] >= 1
+                assert dims["prefix_ranges"] >= 1 and 1 <= dims["own_chunk"] * page <= 2048
                 tiles, group = -(-batch * (hq // hkv) // 128), hq // hkv
-                blocks = -(-hkv * dims["prefix_ranges"] // 8) * 8 * tiles + batch * hkv * -(-group // 16) * dims["own_ranges"]
+                items = -(-own // dims["own_chunk"]) + batch
+                blocks = -(-hkv * dims["prefix_ranges"] // 8) * 8 * tiles + items * -(-hkv // 4) * -(-group // 16)
                 assert eval_extent(manifest["launches"][0]["grid"][0], dims) == blocks
-                items = next(p for p in manifest["params"] if p["name"] == "Partial_PM_split")["shape"][0]
-                assert eval_extent(items, dims) == batch * (dims["prefix_ranges"] + dims["own_ranges"])
+                rows = next(p for p in manifest["params"] if p["name"] == "Partial_PM_split")["shape"][0]
+                assert eval_extent(rows, dims) == batch * dims["prefix_ranges"] + items
 
 
 def test_reference_of_shared_pages():

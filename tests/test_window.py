@@ -12,12 +12,12 @@ from cleave_amd.codegen import HipCodeGen
 from cleave_amd.core.errors import CodegenError, SpecError
 from cleave_amd.dynamic import OPERATORS, reference
 from cleave_amd.dynamic.paging import (PAGED_DECODE, RAGGED_PREFILL_CAUSAL, CombineTiling, DenseAttention, PagingSpec, build_split_decode)
-from cleave_amd.dynamic.paging.apply import _paged_outputs, _paged_params, _plan, _prefill_plan
+from cleave_amd.dynamic.paging.apply import _paged_outputs, _paged_params, _plan, _prefill_plan, window_ranges_expr
 from cleave_amd.dynamic.paging.errors import InvalidSpec, UnsupportedTiling
 from cleave_amd.frontend.paged import PagedProgram, trace_paged
 from cleave_amd.pipeline.dynamic import PagedKernel
 from cleave_amd.runtime import shim
-from cleave_amd.runtime.compile import code_object_stats
+from cleave_amd.runtime.compile import code_object_stats, eval_extent
 
 
 @pytest.mark.parametrize("fn", [C.paged_decode_op(window=100, sinks=4), C.paged_decode_op(page=1, window=7), C.prefill_op(window=64, sinks=1),
@@ -94,6 +94,8 @@ def _decode_plan(window, sinks=0, d=128, **kw):
 def test_kernels_compile_without_spills():
     spec, dense, plan = _decode_plan(100, 4)
     sources = [HipCodeGen().gen(plan), HipCodeGen().gen(build_split_decode(spec, dense, 4, CombineTiling(split=4)))]
+    items = DenseAttention(16, 32, 128, 128, "float16", "float16", waves=2, chunk_pages=-1, lockstep=True)
+    sources.append(HipCodeGen().gen(build_split_decode(spec, items, 4, CombineTiling(split=4))))
     prefill = PagingSpec(8, 2, kind=RAGGED_PREFILL_CAUSAL, causal=True, window=100, sinks=4, cache_inputs=("K", "V"))
     for d in (64, 128, 256):
         sources.append(HipCodeGen().gen(_prefill_plan(prefill, DenseAttention(16, 32, d, 128, "bfloat16", "bfloat16", waves=2))))
@@ -110,11 +112,28 @@ def test_forms_that_have_no_window_are_refused():
         _prefill_plan(prefill, DenseAttention(16, 32, 384, 128, "bfloat16", "bfloat16"))
     spec = PagingSpec(8, 2, kind=PAGED_DECODE, window=100)
     with pytest.raises(UnsupportedTiling, match="window"):
-        build_split_decode(spec, DenseAttention(16, 32, 128, 128, "float16", "float16", waves=2, chunk_pages=32), 4, CombineTiling(split=4))
-    with pytest.raises((CodegenError, UnsupportedTiling)):
-        spec, dense, plan = _decode_plan(100)
-        plan.role, plan.tiling["CHUNK_PAGES"], plan.split_factor = "partial", 32, 4
+        build_split_decode(spec, DenseAttention(16, 32, 128, 128, "float16", "float16", waves=2, chunk_pages=-2), 4, CombineTiling(split=4))
+    plan = _decode_plan(100)[2]
+    plan.tiling["LOCKSTEP"] = 1
+    with pytest.raises(CodegenError, match="chunked items"):
         HipCodeGen().gen(plan)
+
+
+@pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (31, 33), (2048, 0), (5000, 700), (100000, 4)])
+@pytest.mark.parametrize("ranges", [-1, 1, 7])
+def test_ranges_of_a_window(window, sinks, ranges):
+    """Whatever the request's length, a range's rows fit an item's LDS."""
+    expr = window_ranges_expr(PagingSpec(8, 2, kind=PAGED_DECODE, window=window, sinks=sinks), ranges)
+    for batch in (1, 3, 64, 5000):
+        n = eval_extent(expr, {"batch": batch})
+        assert n >= 1
+        for length in (0, 1, window - 1, window, window + 1, window + sinks, window + 31, window + sinks + 65, 3 * window + 2 * sinks + 5):
+            sink_steps = -(-sinks // 32)
+            skip = max(0, max(0, length - window) // 32 - sink_steps)
+            steps = -(-length // 32) - skip
+            assert steps >= 0 and -(-steps // n) * 32 <= 2048
+            seen = {t for s in range(steps) for t in range(32 * (s if s < sink_steps else s + skip), 32 * (s if s < sink_steps else s + skip) + 32)}
+            assert all(t in seen for t in range(length) if t >= length - window or t < sinks)
 
 
 def test_dispatch_counts_the_tokens_that_are_seen():
