@@ -232,20 +232,29 @@ def _plan(spec, dense, role, params, operands, split=None) -> KernelPlan:
 
 
 # ----------------------------------------------------------------------------- decode over shared pages
-def shared_ranges(spec: PagingSpec) -> list:
-    """Launch-time cuts: the number of ranges of the shared keys, and the table entries of an item of the requests' own: two
-    workgroups on every compute unit, ranges and items of four steps or more."""
+def shared_ranges(spec: PagingSpec, head_dim: int) -> list:
+    """Launch-time cuts: the number of ranges that the shared keys are cut into, and the table entries of an item of the requests' own.
+
+    The workgroups of the shared keys come first and take part of the chip's 512 places, the own keys' fill the others and what falls
+    free.  A step of the former (32 keys, 128 rows) takes 0.62 us, and the own keys about 16 bytes of a place a ns: the former get the
+    twice the share of the places that their work is of both (fewer end later than the own keys do), in ranges of two
+    steps or more.  Partial and sum, us, f16, 64 requests of up to 1024 own keys behind 8192 by (ranges, pages an item): (4, 2) 58.7, (8, 2)
+    46.6, (12, 2) 46.4, (16, 2) 48.7, (32, 2) 59.4, (8, 8) 53.1, (8, 16) 61.7; bf16, 200 of 700 behind 32768: (2, 2) 319, (4, 2) 200, (6, 2) 178,
+    (9, 2) 180, (18, 2) 190.  Own keys ahead of the shared ones 53.7 and 188, both kinds in turn 49.2 and 222: a compute unit's shared keys
+    then wait for their loads behind its own keys'.  Items: as many workgroups as give every place two, of a step or more."""
     from ...core.target import current_target
 
-    resident = 2 * current_target().arch.compute_units
-    b = spec.batch_dim
-    prefix = (f"max(1, min(ceildiv({spec.shared_dim} * {spec.page_size}, {4 * KV_STEP}), "
-              f"{resident} // ({spec.num_kv_heads} * max(1, ceildiv({b} * {spec.group}, 128)))))")
-    pieces = -(-spec.num_kv_heads // 4) * -(-spec.group // 16)                  # workgroups of an item
-    most = max(1, MAX_CHUNK_TOKENS // spec.page_size)
-    least = max(1, 4 * KV_STEP // spec.page_size)
-    own = f"max({min(least, most)}, min({most}, ceildiv({spec.index_dim} * {pieces}, {resident})))"
-    return [("prefix_ranges", prefix), ("own_chunk", own)]
+    places = 2 * current_target().arch.compute_units
+    b, page = spec.batch_dim, spec.page_size
+    steps = f"ceildiv({spec.shared_dim} * {page}, {KV_STEP})"
+    pairs = f"({spec.num_kv_heads} * max(1, ceildiv({b} * {spec.group}, 128)))"            # (kv head, 128 rows)
+    shared = f"({pairs} * {steps})"
+    own = f"({spec.index_dim} * {page} * {spec.num_kv_heads * head_dim} // 1766)"           # in steps of the former
+    prefix = f"max(1, min({steps} // 2, {places} // {pairs}, {2 * places} * {shared} // max(1, {shared} + {own}) // {pairs}))"
+    pieces = -(-spec.num_kv_heads // 4) * -(-spec.group // 16)                               # workgroups of an item
+    most = max(1, MAX_CHUNK_TOKENS // page)
+    chunk = f"max({-(-KV_STEP // page)}, min({most}, ceildiv({spec.index_dim} * {pieces}, {2 * places})))"
+    return [("prefix_ranges", prefix), ("own_chunk", chunk)]
 
 
 def _shared_plan(spec: PagingSpec, dense: DenseAttention) -> KernelPlan:
@@ -266,7 +275,7 @@ def _shared_plan(spec: PagingSpec, dense: DenseAttention) -> KernelPlan:
     problem = _paged_problem(spec, dense)
     problem["dim_names"] = {"batch": b, "num_pages": spec.pages_dim, "n_idx": spec.index_dim, "n_shared": spec.shared_dim}
     return KernelPlan(template="attn_shared", role="main", family="attention", dtype=dense.dtype,
-                      extra={"derived_dims": shared_ranges(spec)}, problem=problem, tiling={}, params=params + outs,
+                      extra={"derived_dims": shared_ranges(spec, dense.head_dim)}, problem=problem, tiling={}, params=params + outs,
                       operands={**operands, **out_ops}, split_factor=None, dyn_dims=tuple(problem["dim_names"].values()), n_threads=256,
                       label=f"shared pages kv={KV_STEP} q=128 thr=256")
 

@@ -99,7 +99,7 @@ def test_launch_time_cuts(hq, hkv, page):
     plan's arithmetic is the manifest's."""
     spec = spec_of(page, hq, hkv)
     manifest = _load_main_kernel_from_code(HipCodeGen().gen(_shared_plan(spec, DenseAttention(-(-hq // hkv // 16) * 16, 32, 128, 256, "float16", "float16")))).manifest
-    assert [list(r) for r in shared_ranges(spec)] == manifest["derived_dims"]
+    assert [list(r) for r in shared_ranges(spec, 128)] == manifest["derived_dims"]
     for batch in (1, 2, 7, 64, 300, 5000):
         for shared in (0, 1, 100, 40000):
             for own in (0, 1, 777, 300000):
