@@ -500,17 +500,18 @@ class HipCodeGen:
         params[at:at] = scratch
         return dataclasses.replace(plan, role="fused", operands=operands, split_factor=keys)
 
-    def _launch_chunk_combine(self, unit, rows, vdim, items):
+    def _launch_chunk_combine(self, unit, rows, vdim, items, only=None):
         """The launch that merges the partials of chunked items: groups of threads share the items of a row where one thread per four
-        columns would be fewer workgroups than there are ``items`` (the kernel makes the same choice)."""
+        columns would be fewer workgroups than there are ``items`` (the kernel makes the same choice).  ``only``: a factor of 1 or 0, the
+        latter in calls that have nothing to merge."""
         from ..schedule.policy import COMBINE_GROUPS
 
         groups = next(n for n in COMBINE_GROUPS if vdim * n % 1024 == 0)
         unit.define("CL_COMBINE_GROUPS", groups)
         plain = f"ceildiv({rows} * {vdim // 4}, 256)"
         grouped = f"min(max({items} - {plain}, 0), 1)"
-        unit.launch(self._combine_args[0], (f"{plain} + ({rows} * {vdim * groups // 1024} - {plain}) * {grouped}", 1, 1), 256, 0,
-                    self._combine_args[1])
+        grid = f"{plain} + ({rows} * {vdim * groups // 1024} - {plain}) * {grouped}"
+        unit.launch(self._combine_args[0], (f"({grid}) * {only}" if only else grid, 1, 1), 256, 0, self._combine_args[1], optional=only is not None)
 
     def _launch_combine(self, unit, rows, vdim, splits, po_elem=False, plain=None):
         """The launch that merges the f32 (or, ``po_elem``, element-type) partials of ``splits`` key ranges.
@@ -713,8 +714,12 @@ class HipCodeGen:
         p, op = plan.problem, plan.operands
         if combine or (plan.split_factor or 1) > 1:
             raise CodegenError("prefill has no split-KV form")
-        emit_lse = bool(p.get("emit_lse"))
-        self._attn_common(unit, plan, params, partial, combine, fused, p["vdim"], f"(total_q * {p['q_heads']})", emit_lse)
+        emit_lse, windowed = bool(p.get("emit_lse")), bool(p.get("window"))
+        self._attn_common(unit, plan, params, partial, windowed, fused, p["vdim"], f"(total_q * {p['q_heads']})", emit_lse)
+        if windowed:
+            unit.define("CL_ITEM_RANGES", "ranges")
+            for role in ("PM", "PL", "PO"):
+                unit.define(f"CL_ARG_{role}", op[role])
         d, group = p["head_dim"], p["group"]
         if d % 32 or not (d % 128 == 0 or d == 64) or 16 % group or p["kv_heads"] > 16:
             raise CodegenError("prefill needs head_dim 64 or k*128, a head group dividing 16 and at most 16 kv heads")
@@ -736,7 +741,11 @@ class HipCodeGen:
             # the item axis is padded to a multiple of 8 so that the kernel can hand every XCD one
             # contiguous eighth of the (kv head, item) space
             items = f"ceildiv(ceildiv({p['dim_names']['total_q']}, {128 // group}) + batch, 8) * 8"
-            unit.launch(ENTRY, (items, p["kv_heads"], 1), 256, 0, self._partial_args)
+            unit.launch(ENTRY, (items, p["kv_heads"], "ranges" if windowed else 1), 256, 0, self._partial_args)
+            if windowed:
+                unit.templates.append("attn_combine.hip")
+                tq = p["dim_names"]["total_q"]
+                self._launch_chunk_combine(unit, f"({tq} * {p['q_heads']})", p["vdim"], f"{tq} * ranges", only="min(ranges - 1, 1)")
             return
         unit.templates.append("attn_prefill.hip")
         items = f"ceildiv({p['dim_names']['total_q']}, {16 // group}) + batch"

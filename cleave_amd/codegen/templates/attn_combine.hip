@@ -26,7 +26,7 @@ CL_DEVICE void cb_store(float m, float l, f32x4 o, elem_t* out, float* lse) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) r[i] = to_elem(o[i] * inv);
   *reinterpret_cast<elem4*>(out) = r;
-  if (lse) *lse = l > 0.f ? m + fast_log2(l) : CL_NEG_INF;
+  if (lse) *lse = cl_lse(m, l);
 }
 // Adds a partial of weight f to a row's sums, or, of a slot past the last partial, nothing.  (Weight 0 is not nothing: a partial may hold
 // infinite values.)
@@ -201,7 +201,7 @@ CL_COMBINE_NAME(CL_COMBINE_PARAMS) {
   for (int i = 0; i < 8; ++i) r[i] = to_elem(o[i] * inv);
   st16(CL_CARG_OUT + row * CL_VDIM + d, as_u32x4(r));
 #if CL_EMIT_LSE
-  if (d == 0) CL_CARG_LSE[row] = l > 0.f ? m + fast_log2(l) : CL_NEG_INF;
+  if (d == 0) CL_CARG_LSE[row] = cl_lse(m, l);
 #endif
 }
 #elif CL_SPLITS > 1 && CL_EMIT_COMBINE && CL_COMBINE_GROUPS > 1
@@ -266,7 +266,7 @@ CL_COMBINE_NAME(CL_COMBINE_PARAMS) {
   for (int i = 0; i < 4; ++i) r[i] = to_elem(o[i] * inv);
   *reinterpret_cast<elem4*>(CL_CARG_OUT + row * CL_VDIM + d) = r;
 #if CL_EMIT_LSE
-  if (d == 0) CL_CARG_LSE[row] = l > 0.f ? m + fast_log2(l) : CL_NEG_INF;
+  if (d == 0) CL_CARG_LSE[row] = cl_lse(m, l);
 #endif
 }
 #endif

@@ -92,6 +92,12 @@
 #if CL_SKEW && (CL_CHUNK_PAGES || CL_SPLITS % 2)
 #error "skewed split ranges: an even number of splits, no chunked items"
 #endif
+// (under a window and over shared pages an undefined score makes its row undefined; elsewhere its key is left out)
+#if CL_WINDOW || CL_OWN_PART
+#define ATT_WEIGHS(s) (!((s) <= 0.5f * CL_NEG_BIG))
+#else
+#define ATT_WEIGHS(s) ((s) > 0.5f * CL_NEG_BIG)
+#endif
 #define ATT_STEP 32
 #if CL_WINDOW
 #define ATT_SINK_STEPS ((CL_SINKS + ATT_STEP - 1) / ATT_STEP)
@@ -551,7 +557,7 @@ _Pragma("unroll")                                                               
       float psum = 0.f;                                                                             \
 _Pragma("unroll")                                                                                   \
       for (int i = 0; i < 8; ++i) {                                                                 \
-        float p = s[i] > 0.5f * CL_NEG_BIG ? fast_exp2(s[i] - m_new) : 0.f;                         \
+        float p = ATT_WEIGHS(s[i]) ? fast_exp2(s[i] - m_new) : 0.f;                                 \
         psum += p;                                                                                  \
         pf[i] = to_elem(p);                                                                         \
       }                                                                                             \
@@ -683,7 +689,7 @@ _Pragma("unroll")                                                               
       CL_ARG_PM[prow] = m_run;
       CL_ARG_PL[prow] = l_run;
 #elif CL_EMIT_LSE
-      CL_ARG_LSE[orow] = l_run > 0.f ? m_run + fast_log2(l_run) : CL_NEG_INF;
+      CL_ARG_LSE[orow] = cl_lse(m_run, l_run);
 #endif
     }
   }

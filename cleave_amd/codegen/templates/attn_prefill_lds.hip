@@ -65,7 +65,12 @@
 //
 // CL_WINDOW, CL_SINKS (paged modes): a row sees the last CL_WINDOW keys up to its own and the request's first CL_SINKS ones.
 // Steps are numbered without the ones that no row of the item sees: step s is 32-key tile s of the request up to the sinks' last
-// tile and tile s + skip behind it; tiles that a row of the wave sees in part are masked at either end.
+// tile and tile s + skip behind it; tiles that a row of the wave sees in part are masked at either end.  An item's steps are dealt
+// out to `ranges` (a run-time argument, grid.z) equal parts: one, or where there are too few items for the chip several, which
+// write f32 partials (query token, range, query head[, d]) for attn_combine.hip.
+// A masked key has weight 0, and 0 times a value that is not finite is not 0: a wave that meets such a value in a step that
+// it masks takes its rows again at the end, key by key over what each sees (a handful of instructions a masked step beside; keys
+// ahead of the item's windows, whose rows a cache may have given away, are not read).
 //
 //   CL_HEAD_DIM (multiple of 64)  CL_KV_HEADS  CL_Q_HEADS (group divides 16)  CL_RAGGED
 //   run-time: batch, total_q, n_idx (table length / total_kv), num_pages (table form), sm_scale
@@ -110,6 +115,13 @@
 #if CL_SPLITS > 1 && !CL_DENSE && !CL_PREFIX
 #error "split keys: dense operands and shared pages only"
 #endif
+#if CL_WINDOW
+#define PL_PART (ranges > 1)                  // this workgroup writes partials
+#define PL_PARTIALS 1
+#else
+#define PL_PART (CL_SPLITS > 1)
+#define PL_PARTIALS (CL_SPLITS > 1)
+#endif
 #if CL_PREFIX
 #define PL_TABLE CL_ARG_SHARED
 #define PL_PROW(split, m) ((((i64)(lo + (m)) / PL_GROUP) * prefix_ranges + (split)) * CL_Q_HEADS + head * PL_GROUP + (lo + (m)) % PL_GROUP)
@@ -117,7 +129,11 @@
 #define PL_ROW(page, pos) ((page) * CL_PAGE_SIZE + (pos) % CL_PAGE_SIZE)
 #else
 #define PL_TABLE CL_ARG_INDICES
+#if CL_WINDOW
+#define PL_PROW(split, m) ((((i64)lo + (m) / PL_GROUP) * ranges + (split)) * CL_Q_HEADS + head * PL_GROUP + (m) % PL_GROUP)
+#else
 #define PL_PROW(split, m) ((i64)(split) * CL_TOTAL_ROWS + row_index(m))
+#endif
 #define PL_PAGE(pos) (pos)
 #define PL_ROW(page, pos) (page)
 #endif
@@ -255,8 +271,26 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
     limit[rt] = live[rt] ? row_limit(m) : -1;
   }
 
-#if CL_SPLITS > 1
-  if (ext == 0) {
+#if CL_WINDOW
+  // the item's first row begins its window first
+  constexpr int sink_steps = (CL_SINKS + PL_STEP - 1) / PL_STEP;
+  int skip, first_step, n_steps;
+  const int first_key = off + (lo - q0) - CL_WINDOW + 1;
+  {
+    skip = (first_key > 0 ? first_key : 0) / PL_STEP - sink_steps;
+    skip = skip > 0 ? skip : 0;
+    const int all = (ext + PL_STEP - 1) / PL_STEP - skip, each = (all + ranges - 1) / ranges;
+    first_step = (int)blockIdx.z * each;
+    n_steps = all - first_step < each ? all - first_step : each;
+  }
+  const int split = blockIdx.z;
+#else
+  constexpr int sink_steps = 0, skip = 0, first_step = 0;
+  const int n_steps = (ext + PL_STEP - 1) / PL_STEP;
+#endif
+  auto tile_of = [&](int s) __attribute__((always_inline)) { return CL_WINDOW && s + first_step >= sink_steps ? s + first_step + skip : s + first_step; };
+#if PL_PARTIALS
+  if (PL_PART && n_steps <= 0) {
     // a range past the last key: the partial of nothing
 #pragma unroll
     for (int rt = 0; rt < 2; ++rt) {
@@ -272,7 +306,8 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
     }
     return;
   }
-#else
+#endif
+#if CL_SPLITS == 1
   if (ext == 0) {
     // no row of the item sees a key: zeros and -inf, nothing to read
 #pragma unroll
@@ -304,17 +339,6 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
   const char* kbase = reinterpret_cast<const char*>(CL_ARG_K) + (i64)head * CL_HEAD_DIM * 2;
   const char* vbase = reinterpret_cast<const char*>(CL_ARG_V) + (i64)head * CL_VDIM * 2;
 #endif
-#if CL_WINDOW
-  // (the item's first row begins its window first)
-  constexpr int sink_steps = (CL_SINKS + PL_STEP - 1) / PL_STEP;
-  const int first_key = off + (lo - q0) - CL_WINDOW + 1;
-  int skip = (first_key > 0 ? first_key : 0) / PL_STEP - sink_steps;
-  skip = skip > 0 ? skip : 0;
-#else
-  constexpr int sink_steps = 0, skip = 0;
-#endif
-  auto tile_of = [&](int s) __attribute__((always_inline)) { return CL_WINDOW && s >= sink_steps ? s + skip : s; };
-  const int n_steps = (ext + PL_STEP - 1) / PL_STEP - skip;
   const unsigned tiles_byte = (unsigned)(size_t)(__attribute__((address_space(3))) elem_t*)pl_tiles;
 
   // Loads of one step, this wave's share: key rows 8 wave + lane / 8 of every 64-feature panel, the chunk for slot
@@ -322,7 +346,7 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
   // same number of loads at every wait; positions past the item's last key repeat it.
   const int my_r = 8 * wave + (lane >> 3);
   const int chunk_byte = 16 * ((lane & 7) ^ pl_swz(my_r));
-  const int last_step = n_steps - 1, tail_r = ext - 1 - PL_STEP * (last_step + skip);      // last row of the last step
+  const int last_step = n_steps - 1, tail_r = ext - 1 - PL_STEP * tile_of(last_step);      // last row of the last step (31 and more: all)
   const int row_tail = my_r < tail_r ? my_r : tail_r;
 #if CL_RAGGED
   // consecutive rows: a scalar base per step and one of two lane offsets (whole step / last step)
@@ -377,7 +401,12 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
   };
 #if !CL_RAGGED
   auto key_pos = [&](int s) __attribute__((always_inline)) {
-    return PL_STEP * tile_of(s < last_step ? s : last_step) + (s < last_step ? my_r : row_tail);
+    const int at = PL_STEP * tile_of(s < last_step ? s : last_step) + (s < last_step ? my_r : row_tail);
+#if CL_WINDOW
+    return at < first_key && at >= CL_SINKS ? first_key : at;
+#else
+    return at;
+#endif
   };
   auto row_of = [&](int s) __attribute__((always_inline)) {
     const int at = kv0 + key_pos(s);
@@ -443,6 +472,13 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
 #endif
   }
 
+#if CL_WINDOW
+  // The values of masked steps times nothing: NaN from the first one on that is not finite.  (On the matrix cores, which have room:
+  // us, packed prompts of up to 8192 tokens, no check 533, this 545, a dot product of each pair on the vector unit 548.)
+  f32x4 taint = (f32x4){0.f, 0.f, 0.f, 0.f};
+  u32x4 no_bits = (u32x4){0u, 0u, 0u, 0u};
+  const elem8 none = as_elem8(no_bits);
+#endif
   float m_run[2] = {CL_NEG_BIG, CL_NEG_BIG};   // reference point of a row's weights (log2 domain, the row's running max or up to 8 below it), uniform over g
   float l_run[2] = {0.f, 0.f};                 // this lane's share of the sum of the weights
   f32x4 acc[2][PL_FB];                         // acc[rt][fb][r] = O[row][16 fb + 4 g + r]
@@ -477,7 +513,7 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
   int n_full = n_steps;
   if (32 * wave < n_rows) {
     const int first_limit = row_limit(32 * wave);
-    n_full = first_limit < 0 ? 0 : (first_limit + 1) / PL_STEP - skip;
+    n_full = first_limit < 0 ? 0 : (first_limit + 1) / PL_STEP - skip - first_step;
     n_full = n_full < n_steps ? n_full : n_steps;
   }
   n_full = __builtin_amdgcn_readfirstlane(n_full);
@@ -488,7 +524,7 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
   if (32 * wave < n_rows) {
     const int last_row = 32 * wave + 31 < n_rows ? 32 * wave + 31 : n_rows - 1;
     const int begun = row_limit(last_row) - CL_WINDOW + 1;
-    n_low = begun > 0 ? (begun + PL_STEP - 1) / PL_STEP - skip : 0;
+    n_low = begun > 0 ? (begun + PL_STEP - 1) / PL_STEP - skip - first_step : 0;
   }
   n_low = __builtin_amdgcn_readfirstlane(n_low);
 #else
@@ -756,6 +792,13 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
 #pragma unroll
     for (int fb = 0; fb < PL_FB; ++fb) acc[1][fb] = mfma16(vf[fb], pf[1], acc[1][fb]);
     ask(PlC<3>{});
+#if CL_WINDOW
+    // (here: a branch between the products above, whose operands it reads, keeps them from running beside each other, 5 % of a call)
+    if (step >= n_full || step < n_low) {
+#pragma unroll
+      for (int fb = 0; fb < PL_FB; ++fb) taint = mfma16(vf[fb], none, taint);
+    }
+#endif
 #pragma unroll
     for (int rt = 0; rt < 2; ++rt)
 #pragma unroll
@@ -794,6 +837,67 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
   }
   // no load may still be on its way into LDS when the workgroup ends
   PL_WAITCNT(0);
+#if CL_WINDOW
+  const float tainted = (taint[0] + taint[1]) + (taint[2] + taint[3]);
+  if (__builtin_expect(__builtin_amdgcn_ballot_w64(tainted != tainted) != 0, 0)) {
+    // the wave's rows key by key, 64 features at a time: the largest score of what a row sees, then its weights
+    for (int mw = 0; mw < 32; ++mw) {
+      const int m = 32 * wave + mw;
+      if (m >= n_rows) break;
+      const int last = row_limit(m);
+      const i64 row = row_index(m);
+      float q[PL_KPANELS], o[PL_VPANELS], top = CL_NEG_BIG, sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < PL_KPANELS; ++i) q[i] = to_f32(CL_ARG_Q[row * CL_HEAD_DIM + 64 * i + lane]);
+#pragma unroll
+      for (int i = 0; i < PL_VPANELS; ++i) o[i] = 0.f;
+      for (int pass = 0; pass < 2; ++pass)
+        for (int s = 0; s < n_steps; ++s)
+          for (int r = 0; r < PL_STEP; ++r) {
+            const int at = PL_STEP * tile_of(s) + r;
+            if (at > last || (at <= last - CL_WINDOW && at >= CL_SINKS)) continue;
+#if CL_RAGGED
+            const i64 key = kv0 + at;
+#else
+            const i64 key = pl_clamp(CL_ARG_INDICES[kv0 + at], 0, num_pages - 1);
+#endif
+            const elem_t* kr = reinterpret_cast<const elem_t*>(kbase + key * krow_bytes);
+            const elem_t* vr = reinterpret_cast<const elem_t*>(vbase + key * vrow_bytes);
+            float dot = 0.f;
+#pragma unroll
+            for (int i = 0; i < PL_KPANELS; ++i) dot += q[i] * to_f32(kr[64 * i + lane]);
+#pragma unroll
+            for (int b = 1; b < 64; b *= 2) dot += lane_xor(dot, lane, b);
+            const float score = (q_sign ? -dot : dot) * scale2;
+            if (pass == 0) {
+              top = fmaxf(top, score);
+            } else {
+              const float w = fast_exp2(score - top);
+              sum += w;
+#pragma unroll
+              for (int i = 0; i < PL_VPANELS; ++i) o[i] += w * to_f32(vr[64 * i + lane]);
+            }
+          }
+      if (PL_PART) {
+        const i64 prow = PL_PROW(split, m);
+#pragma unroll
+        for (int i = 0; i < PL_VPANELS; ++i) CL_ARG_PO[prow * CL_VDIM + 64 * i + lane] = o[i];
+        if (lane == 0) {
+          CL_ARG_PM[prow] = top;
+          CL_ARG_PL[prow] = sum;
+        }
+      } else {
+        const float inv = 1.0f / fmaxf(sum, 1.0e-30f);
+#pragma unroll
+        for (int i = 0; i < PL_VPANELS; ++i) CL_ARG_OUT[row * CL_VDIM + 64 * i + lane] = to_elem(o[i] * inv);
+#if CL_EMIT_LSE
+        if (lane == 0) CL_ARG_LSE[row] = cl_lse(top, sum);
+#endif
+      }
+    }
+    return;
+  }
+#endif
 
   // ---- each lane writes its rows' features (a row that saw no key: 0 and lse -inf) --------------
   // (row coordinates are worked out again from the lane number, behind a barrier for the
@@ -814,9 +918,9 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
     const float inv = 1.0f / fmaxf(l, 1.0e-30f);
 #endif
     const i64 orow = row_index(m);
-#if CL_SPLITS > 1
+#if PL_PARTIALS
     // split partials: unnormalised f32 values (16 bytes per lane and block), m and l by the g == 0 lanes
-    {
+    if (PL_PART) {
       const i64 prow = PL_PROW(split, m);
       float* dstp = CL_ARG_PO + prow * CL_VDIM + 4 * g_e;
 #pragma unroll
@@ -831,11 +935,13 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
 #endif
       }
       (void)inv;
+      continue;
     }
-#else
+#endif
+#if CL_SPLITS == 1
     pl_store_row<PL_FB, CL_DENSE>(CL_ARG_OUT + orow * CL_VDIM, acc[rt], inv, g_e);
 #if CL_EMIT_LSE
-    if (g_e == 0) CL_ARG_LSE[orow] = l > 0.f ? m_run[rt] + fast_log2(l) : CL_NEG_INF;
+    if (g_e == 0) CL_ARG_LSE[orow] = cl_lse(m_run[rt], l);
 #endif
 #endif
   }

@@ -33,6 +33,15 @@ CL_DEVICE f32x4 mfma16(elem8 a, elem8 b, f32x4 c) {
 
 CL_DEVICE float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 CL_DEVICE float fast_log2(float x) { return __builtin_amdgcn_logf(x); }
+// base-2 log-sum-exp of weights that sum to `l` against the reference point `m`: -inf of none (l == 0), and of undefined weights
+// NaN under a window and over shared pages, -inf elsewhere
+CL_DEVICE float cl_lse(float m, float l) {
+#if CL_WINDOW || CL_OWN_PART
+  return l <= 0.f ? CL_NEG_INF : m + fast_log2(l);
+#else
+  return l > 0.f ? m + fast_log2(l) : CL_NEG_INF;
+#endif
+}
 CL_DEVICE float fast_rsqrt(float x) { return __builtin_amdgcn_rsqf(x); }
 CL_DEVICE float fast_rcp(float x) { return __builtin_amdgcn_rcpf(x); }
 

@@ -324,7 +324,28 @@ def window_ranges_expr(spec, ranges: int) -> str:
 # Parameter order of the reference's operators (``python/cleave/dynamic/reference.py:204-278``):
 # q, k_cache, v_cache, qo_indptr, kv_indptr, kv_indices, sm_scale (token table) or
 # q, k, v, qo_indptr, kv_indptr, sm_scale (packed keys); then out (total_q, heads, d), lse.
-def _prefill_plan(spec: PagingSpec, dense: DenseAttention, shared: bool | None = None, knobs=None) -> KernelPlan:
+def prefill_ranges_expr(spec: PagingSpec, head_dim: int, ranges: int = -1) -> str:
+    """The launch-time number of ranges that an item's keys of a window are dealt out to: the fixed value, or for -1 by what more of them
+    save and cost.  ``r`` ranges save 1 - 1 / r of an item's steps (0.62 us each) and cost a launch and ``r`` times the partials, which are
+    written and read at 3 TB/s: with ``room`` the quotient of the former's steps and the latter's bytes the best number is its root, taken
+    in steps of one, two, four and eight; no more than give every compute unit two workgroups and a range eight steps.  us, bf16, 32 / 8
+    heads, table, window and new tokens by ranges: 4000, 1 x 8 tokens 1 76.1, 4 26.3, 8 22.3, 16 18.4; 1 x 40 1 77.7, 4 29.5, 8 28.4, 16 26.7;
+    2 x 300 1 79.4, 2 70.8, 4 70.7, 8 89.7; 1000, 2 x 300 1 29.8, 2 36.2; 500, 1 x 100 1 18.0, 2 17.3, 8 22.9; packed, 4096, 1 x 2000 1 49.5, 2 70.8."""
+    from ...core.target import current_target
+
+    if ranges > 0:
+        return str(ranges)
+    tokens = 128 // spec.group                                                        # query tokens of an item
+    most = -(-(spec.window + tokens + KV_STEP - 2) // KV_STEP) + -(-spec.sinks // KV_STEP)
+    keys = spec.kv_tokens_dim if spec.kind == RAGGED_PREFILL_CAUSAL else spec.index_dim
+    steps = f"min({most}, ceildiv({keys}, {KV_STEP}))"                                # (no request has more keys than all have)
+    room = f"({steps} * 232500 // max(1, {spec.tokens_dim} * {spec.num_qo_heads * (head_dim + 2)}))"
+    best = f"1 + min(1, {room} // 6) + min(1, {room} // 12) + 2 * min(1, {room} // 24) + 4 * min(1, {room} // 80) + 8 * min(1, {room} // 300)"
+    items = f"(ceildiv({spec.tokens_dim}, {tokens}) + batch)"
+    return f"max(1, min({2 * current_target().arch.compute_units} // max(1, {items} * {spec.num_kv_heads}), min({steps} // 8, {best})))"
+
+
+def _prefill_plan(spec: PagingSpec, dense: DenseAttention, shared: bool | None = None, knobs=None, ranges: int = -1) -> KernelPlan:
     """``shared``: the kernel whose four waves share every key tile through LDS (128 query rows per
     workgroup, for long requests) instead of the one-wave-per-kv-head kernel with 16-row items;
     None: follow the dense tiling (four or more waves ask for the shared form).  ``knobs``: further
@@ -357,6 +378,14 @@ def _prefill_plan(spec: PagingSpec, dense: DenseAttention, shared: bool | None =
     if spec.emit_lse:
         outs.append(ParamSpec("OutputNode_1", "float32", (tq, spec.num_qo_heads), "output"))
         operands["OUT1"] = "OutputNode_1"
+    derived, scratch = [("batch", f"{spec.indptr_dim} - 1")], []
+    if spec.window is not None:
+        # (partials of the ranges of a window's keys, where a call has more than one)
+        derived.append(("ranges", prefill_ranges_expr(spec, d, ranges)))
+        rows = f"max(1, {tq} * ranges * min(ranges - 1, 1))"
+        for role, extents in (("PM", (rows, spec.num_qo_heads)), ("PL", (rows, spec.num_qo_heads)), ("PO", (rows, spec.num_qo_heads, d))):
+            scratch.append(ParamSpec(f"Scratch_{role.lower()}", "float32", extents, "scratch"))
+            operands[role] = operands[f"{role}_COMBINE"] = scratch[-1].name
     # kernel-side names of the run-time extents: the key count is the table length or the packed
     # key rows; the request count follows from the row pointers
     dim_names = {"total_q": tq, "n_idx": spec.kv_tokens_dim} if ragged else \
@@ -366,8 +395,8 @@ def _prefill_plan(spec: PagingSpec, dense: DenseAttention, shared: bool | None =
                "emit_lse": bool(spec.emit_lse), "units": None, "skv": 0, "sq": 0, "scale": 1.0, **_limits(spec), "dim_names": dim_names}
     threads, rows = (256, 128) if shared else (spec.num_kv_heads * 64, 16)
     return KernelPlan(template="attn_prefill", role="main", family="attention", dtype=dense.dtype,
-                      extra={"derived_dims": [("batch", f"{spec.indptr_dim} - 1")]}, problem=problem,
-                      tiling={"SHARED": int(bool(shared)), **(dict(knobs or {}) if shared else {})}, params=params + outs, operands=operands, split_factor=None,
+                      extra={"derived_dims": derived}, problem=problem,
+                      tiling={"SHARED": int(bool(shared)), **(dict(knobs or {}) if shared else {})}, params=params + scratch + outs, operands=operands, split_factor=None,
                       dyn_dims=tuple(dim_names.values()), n_threads=threads, label=f"kv={KV_STEP} q={rows} thr={threads}")
 
 

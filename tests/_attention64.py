@@ -32,10 +32,16 @@ def attend(q, k, v, scale, seen=None):
     off = d * 2.0 ** -24 * size                                   # of a logit, natural units
     logits = logits.masked_fill(~mask, -math.inf)
     lse = torch.logsumexp(logits, -1, keepdim=True)
-    w = torch.where(mask, torch.exp(logits - lse), torch.zeros_like(logits)).nan_to_num(0)
-    clean = torch.where(mask.any(1).reshape(1, keys, 1), v64, torch.zeros_like(v64))     # (what nobody sees is not read)
+    w = torch.where(mask & (logits != -math.inf), torch.exp(logits - lse), torch.zeros_like(logits))
+    # (a value that is not finite: the rows that see its key, by what it is; others by the finite values)
+    clean = torch.where(v64.isfinite(), v64, torch.zeros_like(v64))
     out = torch.bmm(w, clean)
-    spread = torch.bmm(w, clean.abs())
+    sees = mask.double().expand(kv, -1, -1).contiguous()
+    for flag, value in ((v64 == math.inf, math.inf), (v64 == -math.inf, -math.inf), (v64.isnan(), math.nan)):
+        if bool(flag.any()):
+            out = torch.where(torch.bmm(sees, flag.double()) > 0, out + value, out)
+    out = torch.where(w.isnan().any(-1, keepdim=True), torch.full_like(out, math.nan), out)
+    spread = torch.bmm(w.nan_to_num(0), clean.abs())
     rel = half + 2 * off + 4e-6 + keys * 2.0 ** -24
     tiny = (2.0 ** -25 * keys if q.dtype == torch.float16 else 0.0) * clean.abs().amax()
     tol = rel * spread + tiny

@@ -124,6 +124,10 @@ def test_infinite_values_of_either_part():
     args[2][args[5][60], 0, 0, 9] = -math.inf                 # the third request's
     print("shared prefix: infinite values", flush=True)
     check(shared_kernel(page), args, lens, page)
+    args[1][args[5][3], 0, 0, 0] = math.nan                   # a key of the first request's own
+    check(shared_kernel(page), args, lens, page)
+    args[1][args[3][1], 0, 1, 0] = math.nan                   # a shared one
+    check(shared_kernel(page), args, lens, page)
 
 
 def test_replayed_beside_eager_calls():

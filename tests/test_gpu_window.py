@@ -134,6 +134,22 @@ def test_decode_never_reads_what_is_not_seen(page, split, ranges, value):
     same(lse, want[1], want[3], "lse")
 
 
+@pytest.mark.parametrize("page", [1, 64])
+@pytest.mark.parametrize("split,ranges", [(None, 0), (8, 0), (2, -1), (2, 3)])
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+def test_decode_values_that_are_not_finite(page, split, ranges, value):
+    """A seen value shows in its feature of its kv head's rows; a seen key that is undefined makes them undefined."""
+    lens, window, sinks = [700, 90, 333], 100, 3
+    args = decode_args(lens, page)
+    for b, (position, head, feature) in enumerate(((650, 0, 5), (1, 1, 9), (333 - 100, 1, 127))):
+        page_of, slot = dref.paged_tokens(args[4], int(args[3][b]), lens[b], page)
+        args[2][page_of[position], slot[position], head, feature] = value
+        if b == 2 and math.isnan(value):
+            args[1][page_of[position + 1], slot[position + 1], 0, 3] = value
+    print(f"window decode not finite {value} page={page} split={split} ranges={ranges}", flush=True)
+    check_decode(decode_kernel(page, window, sinks, split=split, ranges=ranges), args, lens, page, window, sinks)
+
+
 def test_decode_window_of_everything_is_plain_decode():
     lens = [200, 1, 0, 77]
     args = decode_args(lens, 64, hq=32, hkv=8)
@@ -144,11 +160,11 @@ def test_decode_window_of_everything_is_plain_decode():
 
 
 # ------------------------------------------------------------------------------------------------ prompts
-def prefill_kernel(ragged, window, sinks, hq=8, hkv=2, d=128, dtype="bfloat16"):
+def prefill_kernel(ragged, window, sinks, hq=8, hkv=2, d=128, dtype="bfloat16", ranges=-1):
     kind = RAGGED_PREFILL_CAUSAL if ragged else PAGED_PREFILL_CAUSAL
     spec = PagingSpec(hq, hkv, kind=kind, causal=True, window=window, sinks=sinks, **(dict(cache_inputs=("K", "V")) if ragged else {}))
     spec.validate()
-    return compiled(HipCodeGen().gen(_prefill_plan(spec, DenseAttention(16, 32, d, hkv * 64, dtype, dtype, waves=hkv))))
+    return compiled(HipCodeGen().gen(_prefill_plan(spec, DenseAttention(16, 32, d, hkv * 64, dtype, dtype, waves=hkv), ranges=ranges)))
 
 
 def prefill_args(ragged, new, keys, hq=8, hkv=2, d=128, dtype=torch.bfloat16, seed=0):
@@ -182,22 +198,57 @@ KEYS = [1, 40, 5, 33, 9, 200, 3, 130, 1000]      # equal, cached keys, no querie
 
 
 @pytest.mark.parametrize("ragged", [False, True], ids=["table", "packed"])
+@pytest.mark.parametrize("ranges", [-1, 1, 2, 7])
 @pytest.mark.parametrize("window,sinks", [(1, 0), (1, 2), (31, 0), (32, 4), (33, 32), (64, 33), (100, 0), (97, 100), (5000, 4), (40, 500)])
-def test_prefill(ragged, window, sinks):
-    print(f"window prefill ragged={ragged} window={window} sinks={sinks}", flush=True)
+def test_prefill(ragged, ranges, window, sinks):
+    print(f"window prefill ragged={ragged} ranges={ranges} window={window} sinks={sinks}", flush=True)
     args = prefill_args(ragged, NEW, KEYS)
-    check_prefill(prefill_kernel(ragged, window, sinks), args, prefill_want(args, ragged, NEW, KEYS, window, sinks))
+    check_prefill(prefill_kernel(ragged, window, sinks, ranges=ranges), args, prefill_want(args, ragged, NEW, KEYS, window, sinks))
 
 
 @pytest.mark.parametrize("kw", [dict(hq=16, hkv=2), dict(hq=4, hkv=2), dict(d=64), dict(d=256), dict(dtype="float16", hq=32, hkv=8)],
                          ids=lambda kw: "_".join(f"{k}{v}" for k, v in kw.items()))
+@pytest.mark.parametrize("ranges", [1, 3])
 @pytest.mark.parametrize("ragged", [False, True], ids=["table", "packed"])
-def test_prefill_forms(kw, ragged):
+def test_prefill_forms(kw, ragged, ranges):
     new, keys = [150, 3, 70], [150, 900, 333]
     shape = {k: v for k, v in kw.items() if k != "dtype"}
     args = prefill_args(ragged, new, keys, dtype=getattr(torch, kw.get("dtype", "bfloat16")), **shape)
     print(f"window prefill {kw} ragged={ragged}", flush=True)
-    check_prefill(prefill_kernel(ragged, 77, 3, **kw), args, prefill_want(args, ragged, new, keys, 77, 3))
+    check_prefill(prefill_kernel(ragged, 77, 3, ranges=ranges, **kw), args, prefill_want(args, ragged, new, keys, 77, 3))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("ranges", [1, 3])
+@pytest.mark.parametrize("ragged", [False, True], ids=["table", "packed"])
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+def test_prefill_values_that_are_not_finite(ragged, ranges, value, dtype):
+    """Such a value shows in the rows that see its key and in no other, whichever of them share its tile; a key that is not finite
+    makes the rows undefined that see it."""
+    new, keys, window, sinks = [150, 3, 70], [150, 900, 333], 50, 3
+    args = prefill_args(ragged, new, keys, dtype=dtype)
+    at = torch.arange(sum(keys), device="cuda") if ragged else args[5].long()
+    k, v = (t if ragged else t[:, 0] for t in args[1:3])
+    for position, head, feature in ((1, 0, 5), (60, 1, 9), (149, 0, 127), (150 + 897, 1, 64), (150 + 500, 0, 3), (1050 + 280, 1, 1)):
+        v[at[position], head, feature] = value
+    if math.isnan(value):
+        k[at[100], 0, 7] = value
+    print(f"window prefill not finite {value} ragged={ragged} ranges={ranges}", flush=True)
+    check_prefill(prefill_kernel(ragged, window, sinks, ranges=ranges, dtype=str(dtype)[6:]), args, prefill_want(args, ragged, new, keys, window, sinks))
+
+
+@pytest.mark.parametrize("value", [math.inf, math.nan])
+def test_prefill_never_reads_what_no_row_of_an_item_sees(value):
+    """Through a table: entries of tokens ahead of the window lead to rows that are somebody else's by now."""
+    new, keys, window, sinks = [40, 9], [700, 333], 100, 3
+    args = prefill_args(False, new, keys)
+    want = prefill_want(args, False, new, keys, window, sinks)
+    base = 0
+    for n, m in zip(new, keys):
+        hidden = args[5][base + sinks:base + m - n - window + 1].long()
+        args[1][hidden], args[2][hidden] = value, value
+        base += m
+    check_prefill(prefill_kernel(False, window, sinks), args, want)
 
 
 def test_prefill_window_of_everything_is_plain_prefill():
@@ -205,7 +256,7 @@ def test_prefill_window_of_everything_is_plain_prefill():
     args = prefill_args(True, new, keys, hq=32, hkv=8)
     from tests.test_gpu_prefill import prefill_kernel as plain
 
-    for a, b in zip(prefill_kernel(True, 4096, 0, hq=32, hkv=8)(*args), plain(True, shared=True)(*args)):
+    for a, b in zip(prefill_kernel(True, 4096, 0, hq=32, hkv=8, ranges=1)(*args), plain(True, shared=True)(*args)):
         assert torch.equal(a, b)
 
 
