@@ -72,6 +72,32 @@ CL_DEVICE f32x4 ep_apply(f32x4 v, const elem_t* __restrict__ bias, const elem_t*
   ep_finish<4>(f, bias, res, m, n);
   return (f32x4){f[0], f[1], f[2], f[3]};
 }
+// The same in two halves, for wave tiles of many fragments: the pieces of bias and residual are asked for all at once, ahead of the
+// first use (fragment by fragment every one's wait was in sight: 4096 x 4096 x 1024 with a residual 42.5 us, RES_US this way, the bare
+// product 32.1), and each fragment is finished with what has come.
+CL_DEVICE elem4 ep_piece(const elem_t* __restrict__ row, int n) {
+  if constexpr (CL_N % 4 == 0) return *reinterpret_cast<const elem4*>(row + (n < CL_N ? n : CL_N - 4));
+  elem4 v;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) v[r] = row[n + r < CL_N ? n + r : CL_N - 1];
+  return v;
+}
+CL_DEVICE elem4 ep_bias(const elem_t* __restrict__ bias, int n) {
+#if CL_EPI_BIAS
+  return ep_piece(bias, n);
+#else
+  return (elem4){};
+#endif
+}
+CL_DEVICE const elem_t* ep_res_row(const elem_t* __restrict__ res, int m) { return res + (i64)(m < CL_M ? m : CL_M - 1) * CL_N; }
+CL_DEVICE f32x4 ep_with(f32x4 v, elem4 bias, elem4 res) {
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    v[r] = ep_act(CL_EPI_BIAS ? v[r] + to_f32(bias[r]) : v[r]);
+    if (CL_EPI_RES) v[r] += to_f32(res[r]);
+  }
+  return v;
+}
 #if CL_EPI_BIAS
 #define EP_BIAS CL_ARG_BIAS
 #else

@@ -397,6 +397,18 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
     row_scale[i] = fast_rsqrt(t * (1.0f / CL_K) + CL_EPS);
   }
 #endif
+#if CL_EPI && CL_SPLITS == 1
+  elem4 ep_b[GD_TN], ep_r[TM][GD_TN];
+#pragma unroll
+  for (int j = 0; j < GD_TN; ++j) ep_b[j] = ep_bias(EP_BIAS, n0 + bn + 16 * j + 4 * g);
+#if CL_EPI_RES
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < GD_TN; ++j) ep_r[i][j] = ep_piece(ep_res_row(EP_RES, m0 + am + 16 * i + c), n0 + bn + 16 * j + 4 * g);
+  __builtin_amdgcn_sched_barrier(0);
+#endif
+#endif
 #pragma unroll
   for (int i = 0; i < TM; ++i) {
     const int m = m0 + am + 16 * i + c;
@@ -430,7 +442,7 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
       if (n >= CL_N) continue;
       f32x4 v = gd_acc_read(acc[i][j]);
 #if CL_EPI && CL_SPLITS == 1
-      v = ep_apply(v, EP_BIAS, EP_RES, m, n);
+      v = ep_with(v, ep_b[j], CL_EPI_RES ? ep_r[i][j] : (elem4){});
 #endif
 #if CL_SPLITS > 1
       st_cols4<CL_N>(CL_ARG_PACC + (((i64)split * GD_BATCH + batch) * CL_M + m) * CL_N, n, v);

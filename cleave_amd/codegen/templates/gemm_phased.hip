@@ -345,6 +345,29 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
   const int ec = tid & 15, eg = (tid >> 4) & 3;
   const int ewm = (tid >> 6) / CL_WN, ecol = (tid >> 6) % CL_WN * (GP_HN / CL_WN);
   // ---- epilogue: acc[h][i][v][j][r] = C[m0 + h HM + (the wave's first row of that half) + 16 i + c][n0 + HN v + bn + 16 j + 4 g + r]
+#if CL_EPI && CL_SPLITS == 1
+  // (the residual 16 bytes a lane, as the results leave; the lanes of a pair trade halves below)
+  elem4 ep_b[2][GP_TNH];
+  u32x4 ep_r[2][TMH][2][GP_TNH / 2];
+#pragma unroll
+  for (int v = 0; v < 2; ++v)
+#pragma unroll
+    for (int j = 0; j < GP_TNH; ++j) ep_b[v][j] = ep_bias(EP_BIAS, n0 + GP_HN * v + ecol + 16 * j + 4 * eg);
+#if CL_EPI_RES
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int i = 0; i < (h ? TMH1 : TMH); ++i)
+#pragma unroll
+      for (int v = 0; v < 2; ++v)
+#pragma unroll
+        for (int j = 0; j < GP_TNH; j += 2) {
+          const int n = n0 + GP_HN * v + ecol + 16 * (j + (eg & 1)) + 4 * (eg & 2);
+          ep_r[h][i][v][j / 2] = ld16(ep_res_row(EP_RES, m0 + h * HM + ewm * ((h ? HM1 : HM) / CL_WM) + ec + 16 * i) + (n < CL_N ? n : CL_N - 8));
+        }
+  __builtin_amdgcn_sched_barrier(0);
+#endif
+#endif
 #pragma unroll
   for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -368,11 +391,22 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
 #pragma unroll
         for (int j = 0; j < GP_TNH; j += 2) {
           u32x2 y[2];
+#if CL_EPI
+          u32x2 res[2] = {};
+#if CL_EPI_RES
+          u32x4 both = ep_r[h][i][v][j / 2];
+          u32 r0 = both[0], r1 = both[1], r2 = both[2], r3 = both[3];
+          gp_swap_rows16(r0, r2);
+          gp_swap_rows16(r1, r3);
+          res[0] = (u32x2){r0, r1};
+          res[1] = (u32x2){r2, r3};
+#endif
+#endif
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
             elem4 e;
 #if CL_EPI
-            const f32x4 fin = ep_apply(acc[h][i][v][j + q], EP_BIAS, EP_RES, m, n0 + GP_HN * v + ecol + 16 * (j + q) + 4 * eg);
+            const f32x4 fin = ep_with(acc[h][i][v][j + q], ep_b[v][j + q], __builtin_bit_cast(elem4, res[q]));
 #endif
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
