@@ -237,10 +237,10 @@ def shared_ranges(spec: PagingSpec, head_dim: int) -> list:
 
     The workgroups of the shared keys come first and take part of the chip's 512 places, the own keys' fill the others and what falls
     free.  A step of the former (32 keys, 128 rows) takes 0.62 us, and the own keys about 16 bytes of a place a ns: the former get the
-    twice the share of the places that their work is of both (fewer end later than the own keys do), in ranges of two
+    seven quarters of the share of the places that their work is of both (fewer end later than the own keys do), in ranges of two
     steps or more.  Partial and sum, us, f16, 64 requests of up to 1024 own keys behind 8192 by (ranges, pages an item): (4, 2) 58.7, (8, 2)
     46.6, (12, 2) 46.4, (16, 2) 48.7, (32, 2) 59.4, (8, 8) 53.1, (8, 16) 61.7; bf16, 200 of 700 behind 32768: (2, 2) 319, (4, 2) 200, (6, 2) 178,
-    (9, 2) 180, (18, 2) 190.  Own keys ahead of the shared ones 53.7 and 188, both kinds in turn 49.2 and 222: a compute unit's shared keys
+    (7, 2) 172, (9, 2) 180, (18, 2) 190.  Own keys ahead of the shared ones 53.7 and 188, both kinds in turn 49.2 and 222: a compute unit's shared keys
     then wait for their loads behind its own keys'.  Items: as many workgroups as give every place two, of a step or more."""
     from ...core.target import current_target
 
@@ -250,7 +250,7 @@ def shared_ranges(spec: PagingSpec, head_dim: int) -> list:
     pairs = f"({spec.num_kv_heads} * max(1, ceildiv({b} * {spec.group}, 128)))"            # (kv head, 128 rows)
     shared = f"({pairs} * {steps})"
     own = f"({spec.index_dim} * {page} * {spec.num_kv_heads * head_dim} // 1766)"           # in steps of the former
-    prefix = f"max(1, min({steps} // 2, {places} // {pairs}, {2 * places} * {shared} // max(1, {shared} + {own}) // {pairs}))"
+    prefix = f"max(1, min({steps} // 2, {places} // {pairs}, {places * 7 // 4} * {shared} // max(1, {shared} + {own}) // {pairs}))"
     pieces = -(-spec.num_kv_heads // 4) * -(-spec.group // 16)                               # workgroups of an item
     most = max(1, MAX_CHUNK_TOKENS // page)
     chunk = f"max({-(-KV_STEP // page)}, min({most}, ceildiv({spec.index_dim} * {pieces}, {2 * places})))"
