@@ -37,7 +37,7 @@ LOG2E = 1.4426950408889634
 # The operands that a template moves from global memory straight into LDS in 16-byte pieces.  Such a load needs its pieces
 # at multiples of 16 bytes; everything else is read through registers, which takes any element's address.
 DIRECT_TO_LDS = {"gemm_tile.hip": ("A", "B", "C"), "mla_decode.hip": ("KV", "KPE"), "mla_paged_decode.hip": ("KV", "KPE"),
-                 "mla_decode_duo.hip": ("Q", "QPE", "KV", "KPE"), "mla_prefill_duo.hip": ("Q", "QPE", "KV", "KPE"), "attn_prefill_lds.hip": ("K", "V"),
+                 "mla_decode_duo.hip": ("Q", "QPE", "KV", "KPE"), "mla_prefill_duo.hip": ("Q", "QPE", "KV", "KPE"), "attn_prefill_lds.hip": ("K", "V"), "attn_window.hip": ("K", "V"),
                  "attn_phased.hip": ("K", "V")}
 
 _C_TYPES = {"float16": "elem_t", "bfloat16": "elem_t", "float32": "float", "int32": "int"}
@@ -741,11 +741,13 @@ class HipCodeGen:
             # the item axis is padded to a multiple of 8 so that the kernel can hand every XCD one
             # contiguous eighth of the (kv head, item) space
             items = f"ceildiv(ceildiv({p['dim_names']['total_q']}, {128 // group}) + batch, 8) * 8"
-            unit.launch(ENTRY, (items, p["kv_heads"], "ranges" if windowed else 1), 256, 0, self._partial_args)
             if windowed:
-                unit.templates.append("attn_combine.hip")
+                unit.templates[-1:] = ["attn_window.hip", "attn_combine.hip"]
+                unit.launch(ENTRY, (items, p["kv_heads"], "ranges"), 256, 0, self._partial_args)
                 tq = p["dim_names"]["total_q"]
                 self._launch_chunk_combine(unit, f"({tq} * {p['q_heads']})", p["vdim"], f"{tq} * ranges", only="min(ranges - 1, 1)")
+                return
+            unit.launch(ENTRY, (items, p["kv_heads"], 1), 256, 0, self._partial_args)
             return
         unit.templates.append("attn_prefill.hip")
         items = f"ceildiv({p['dim_names']['total_q']}, {16 // group}) + batch"

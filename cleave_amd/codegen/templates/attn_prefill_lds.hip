@@ -63,15 +63,6 @@
 //
 // CL_PF_XCD / CL_PF_REVERSE (default 1) switch the XCD mapping and the walking order.
 //
-// CL_WINDOW, CL_SINKS (paged modes): a row sees the last CL_WINDOW keys up to its own and the request's first CL_SINKS ones.
-// Steps are numbered without the ones that no row of the item sees: step s is 32-key tile s of the request up to the sinks' last
-// tile and tile s + skip behind it; tiles that a row of the wave sees in part are masked at either end.  An item's steps are dealt
-// out to `ranges` (a run-time argument, grid.z) equal parts: one, or where there are too few items for the chip several, which
-// write f32 partials (query token, range, query head[, d]) for attn_combine.hip.
-// A masked key has weight 0, and 0 times a value that is not finite is not 0: a wave that meets such a value in a step that
-// it masks takes its rows again at the end, key by key over what each sees (a handful of instructions a masked step beside; keys
-// ahead of the item's windows, whose rows a cache may have given away, are not read).
-//
 //   CL_HEAD_DIM (multiple of 64)  CL_KV_HEADS  CL_Q_HEADS (group divides 16)  CL_RAGGED
 //   run-time: batch, total_q, n_idx (table length / total_kv), num_pages (table form), sm_scale
 
@@ -102,25 +93,11 @@
 #ifndef CL_PREFIX
 #define CL_PREFIX 0
 #endif
-#ifndef CL_WINDOW
-#define CL_WINDOW 0
-#define CL_SINKS 0
-#endif
-#if CL_WINDOW && CL_DENSE
-#error "a window: ragged queries"
-#endif
 #if CL_DENSE && !CL_RAGGED
 #error "dense operands have consecutive key rows (CL_RAGGED)"
 #endif
 #if CL_SPLITS > 1 && !CL_DENSE && !CL_PREFIX
 #error "split keys: dense operands and shared pages only"
-#endif
-#if CL_WINDOW
-#define PL_PART (ranges > 1)                  // this workgroup writes partials
-#define PL_PARTIALS 1
-#else
-#define PL_PART (CL_SPLITS > 1)
-#define PL_PARTIALS (CL_SPLITS > 1)
 #endif
 #if CL_PREFIX
 #define PL_TABLE CL_ARG_SHARED
@@ -129,11 +106,7 @@
 #define PL_ROW(page, pos) ((page) * CL_PAGE_SIZE + (pos) % CL_PAGE_SIZE)
 #else
 #define PL_TABLE CL_ARG_INDICES
-#if CL_WINDOW
-#define PL_PROW(split, m) ((((i64)lo + (m) / PL_GROUP) * ranges + (split)) * CL_Q_HEADS + head * PL_GROUP + (m) % PL_GROUP)
-#else
 #define PL_PROW(split, m) ((i64)(split) * CL_TOTAL_ROWS + row_index(m))
-#endif
 #define PL_PAGE(pos) (pos)
 #define PL_ROW(page, pos) (page)
 #endif
@@ -271,26 +244,8 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
     limit[rt] = live[rt] ? row_limit(m) : -1;
   }
 
-#if CL_WINDOW
-  // the item's first row begins its window first
-  constexpr int sink_steps = (CL_SINKS + PL_STEP - 1) / PL_STEP;
-  int skip, first_step, n_steps;
-  const int first_key = off + (lo - q0) - CL_WINDOW + 1;
-  {
-    skip = (first_key > 0 ? first_key : 0) / PL_STEP - sink_steps;
-    skip = skip > 0 ? skip : 0;
-    const int all = (ext + PL_STEP - 1) / PL_STEP - skip, each = (all + ranges - 1) / ranges;
-    first_step = (int)blockIdx.z * each;
-    n_steps = all - first_step < each ? all - first_step : each;
-  }
-  const int split = blockIdx.z;
-#else
-  constexpr int sink_steps = 0, skip = 0, first_step = 0;
-  const int n_steps = (ext + PL_STEP - 1) / PL_STEP;
-#endif
-  auto tile_of = [&](int s) __attribute__((always_inline)) { return CL_WINDOW && s + first_step >= sink_steps ? s + first_step + skip : s + first_step; };
-#if PL_PARTIALS
-  if (PL_PART && n_steps <= 0) {
+#if CL_SPLITS > 1
+  if (ext == 0) {
     // a range past the last key: the partial of nothing
 #pragma unroll
     for (int rt = 0; rt < 2; ++rt) {
@@ -306,8 +261,7 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
     }
     return;
   }
-#endif
-#if CL_SPLITS == 1
+#else
   if (ext == 0) {
     // no row of the item sees a key: zeros and -inf, nothing to read
 #pragma unroll
@@ -339,6 +293,7 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
   const char* kbase = reinterpret_cast<const char*>(CL_ARG_K) + (i64)head * CL_HEAD_DIM * 2;
   const char* vbase = reinterpret_cast<const char*>(CL_ARG_V) + (i64)head * CL_VDIM * 2;
 #endif
+  const int n_steps = (ext + PL_STEP - 1) / PL_STEP;
   const unsigned tiles_byte = (unsigned)(size_t)(__attribute__((address_space(3))) elem_t*)pl_tiles;
 
   // Loads of one step, this wave's share: key rows 8 wave + lane / 8 of every 64-feature panel, the chunk for slot
@@ -346,7 +301,7 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
   // same number of loads at every wait; positions past the item's last key repeat it.
   const int my_r = 8 * wave + (lane >> 3);
   const int chunk_byte = 16 * ((lane & 7) ^ pl_swz(my_r));
-  const int last_step = n_steps - 1, tail_r = ext - 1 - PL_STEP * tile_of(last_step);      // last row of the last step (31 and more: all)
+  const int last_step = n_steps - 1, tail_r = ext - 1 - PL_STEP * last_step;      // last row of the last step
   const int row_tail = my_r < tail_r ? my_r : tail_r;
 #if CL_RAGGED
   // consecutive rows: a scalar base per step and one of two lane offsets (whole step / last step)
@@ -365,7 +320,7 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
       pl_dma16<0>(kbase + ((i64)feat * CL_SKV + s * PL_STEP) * 2 + 16 * piece, dst + (unsigned)(P * PL_PANEL * 2));
     });
 #elif CL_RAGGED
-    const char* base = kbase + (i64)(kv0 + tile_of(s) * PL_STEP) * krow_bytes;
+    const char* base = kbase + (i64)(kv0 + s * PL_STEP) * krow_bytes;
     const unsigned off = s == last_step ? koff[1] : koff[0];
     pl_static_for<decltype(lo_c)::value, decltype(hi_c)::value>([&](auto p) __attribute__((always_inline)) {
       constexpr int P = decltype(p)::value;
@@ -384,7 +339,7 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
     s = s < last_step ? s : last_step;
     const unsigned dst = tiles_byte + (unsigned)((PL_STAGES * PL_KIMG + slot * PL_VIMG) * 2 + wave * 1024);
 #if CL_RAGGED
-    const char* base = vbase + (i64)(kv0 + tile_of(s) * PL_STEP) * vrow_bytes;
+    const char* base = vbase + (i64)(kv0 + s * PL_STEP) * vrow_bytes;
     const unsigned off = s == last_step ? voff[1] : voff[0];
     pl_static_for<decltype(lo_c)::value, decltype(hi_c)::value>([&](auto p) __attribute__((always_inline)) {
       constexpr int P = decltype(p)::value;
@@ -401,12 +356,7 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
   };
 #if !CL_RAGGED
   auto key_pos = [&](int s) __attribute__((always_inline)) {
-    const int at = PL_STEP * tile_of(s < last_step ? s : last_step) + (s < last_step ? my_r : row_tail);
-#if CL_WINDOW
-    return at < first_key && at >= CL_SINKS ? first_key : at;
-#else
-    return at;
-#endif
+    return PL_STEP * (s < last_step ? s : last_step) + (s < last_step ? my_r : row_tail);
   };
   auto row_of = [&](int s) __attribute__((always_inline)) {
     const int at = kv0 + key_pos(s);
@@ -472,13 +422,6 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
 #endif
   }
 
-#if CL_WINDOW
-  // The values of masked steps times nothing: NaN from the first one on that is not finite.  (On the matrix cores, which have room:
-  // us, packed prompts of up to 8192 tokens, no check 533, this 545, a dot product of each pair on the vector unit 548.)
-  f32x4 taint = (f32x4){0.f, 0.f, 0.f, 0.f};
-  u32x4 no_bits = (u32x4){0u, 0u, 0u, 0u};
-  const elem8 none = as_elem8(no_bits);
-#endif
   float m_run[2] = {CL_NEG_BIG, CL_NEG_BIG};   // reference point of a row's weights (log2 domain, the row's running max or up to 8 below it), uniform over g
   float l_run[2] = {0.f, 0.f};                 // this lane's share of the sum of the weights
   f32x4 acc[2][PL_FB];                         // acc[rt][fb][r] = O[row][16 fb + 4 g + r]
@@ -513,23 +456,10 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
   int n_full = n_steps;
   if (32 * wave < n_rows) {
     const int first_limit = row_limit(32 * wave);
-    n_full = first_limit < 0 ? 0 : (first_limit + 1) / PL_STEP - skip - first_step;
+    n_full = first_limit < 0 ? 0 : (first_limit + 1) / PL_STEP;
     n_full = n_full < n_steps ? n_full : n_steps;
   }
   n_full = __builtin_amdgcn_readfirstlane(n_full);
-#if CL_WINDOW
-  // ... and whose window every row has begun before them: the wave's last row begins its own last.  (Of the sinks' tiles before
-  // that all are masked: one of a hundred steps.)
-  int n_low = 0;
-  if (32 * wave < n_rows) {
-    const int last_row = 32 * wave + 31 < n_rows ? 32 * wave + 31 : n_rows - 1;
-    const int begun = row_limit(last_row) - CL_WINDOW + 1;
-    n_low = begun > 0 ? (begun + PL_STEP - 1) / PL_STEP - skip - first_step : 0;
-  }
-  n_low = __builtin_amdgcn_readfirstlane(n_low);
-#else
-  constexpr int n_low = 0;
-#endif
 
   // key fragment of 16-key half h and 32-feature block j out of the K image in stage SLOT: a 16-byte read, which feeds the
   // wave's two row tiles
@@ -622,18 +552,9 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
   auto mask = [&](f32x4 (&sc)[2][2], int step) __attribute__((always_inline)) {
 #pragma unroll
     for (int rt = 0; rt < 2; ++rt) {
-      const int room = lim_rel[rt] - tile_of(step) * PL_STEP;
-#if CL_WINDOW
-      const int sink_room = CL_SINKS - 4 * g - tile_of(step) * PL_STEP;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int at = 16 * (i >> 2) + (i & 3);
-        sc[rt][i >> 2][i & 3] = at <= room && (at > room - CL_WINDOW || at < sink_room) ? sc[rt][i >> 2][i & 3] : CL_NEG_INF;
-      }
-#else
+      const int room = lim_rel[rt] - step * PL_STEP;
 #pragma unroll
       for (int i = 0; i < 8; ++i) sc[rt][i >> 2][i & 3] = 16 * (i >> 2) + (i & 3) <= room ? sc[rt][i >> 2][i & 3] : (CL_LINEAR ? 0.f : CL_NEG_INF);
-#endif
     }
   };
   // the largest of this lane's eight scores of a row (in the compiler's sight: it keeps the wait states between a matrix op
@@ -657,7 +578,7 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
   read_keys(PlC<1>{}, 0);
 #if !CL_LINEAR && CL_HEAD_DIM <= 192
   // (the first reference points, so that the first weights need not be taken twice; the widest heads have no registers for it)
-  if (n_full <= 0 || n_low > 0) mask(st, 0);
+  if (n_full == 0) mask(st, 0);
 #pragma unroll
   for (int rt = 0; rt < 2; ++rt) {
     const float mx = pl_max_over_groups(step_max(st[rt])) * scale2;
@@ -692,7 +613,7 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
       issue_k(step + 4, (S + 4) % PL_STAGES, PlC<LO - VL>{}, PlC<HI - VH>{}, row_k);
     };
     __builtin_amdgcn_sched_barrier(0);
-    if (step >= n_full || step < n_low) mask(st, step);
+    if (step >= n_full) mask(st, step);
     __builtin_amdgcn_sched_barrier(0);
 
     elem8 pf[2];
@@ -792,13 +713,6 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
 #pragma unroll
     for (int fb = 0; fb < PL_FB; ++fb) acc[1][fb] = mfma16(vf[fb], pf[1], acc[1][fb]);
     ask(PlC<3>{});
-#if CL_WINDOW
-    // (here: a branch between the products above, whose operands it reads, keeps them from running beside each other, 5 % of a call)
-    if (step >= n_full || step < n_low) {
-#pragma unroll
-      for (int fb = 0; fb < PL_FB; ++fb) taint = mfma16(vf[fb], none, taint);
-    }
-#endif
 #pragma unroll
     for (int rt = 0; rt < 2; ++rt)
 #pragma unroll
@@ -837,67 +751,6 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
   }
   // no load may still be on its way into LDS when the workgroup ends
   PL_WAITCNT(0);
-#if CL_WINDOW
-  const float tainted = (taint[0] + taint[1]) + (taint[2] + taint[3]);
-  if (__builtin_expect(__builtin_amdgcn_ballot_w64(tainted != tainted) != 0, 0)) {
-    // the wave's rows key by key, 64 features at a time: the largest score of what a row sees, then its weights
-    for (int mw = 0; mw < 32; ++mw) {
-      const int m = 32 * wave + mw;
-      if (m >= n_rows) break;
-      const int last = row_limit(m);
-      const i64 row = row_index(m);
-      float q[PL_KPANELS], o[PL_VPANELS], top = CL_NEG_BIG, sum = 0.f;
-#pragma unroll
-      for (int i = 0; i < PL_KPANELS; ++i) q[i] = to_f32(CL_ARG_Q[row * CL_HEAD_DIM + 64 * i + lane]);
-#pragma unroll
-      for (int i = 0; i < PL_VPANELS; ++i) o[i] = 0.f;
-      for (int pass = 0; pass < 2; ++pass)
-        for (int s = 0; s < n_steps; ++s)
-          for (int r = 0; r < PL_STEP; ++r) {
-            const int at = PL_STEP * tile_of(s) + r;
-            if (at > last || (at <= last - CL_WINDOW && at >= CL_SINKS)) continue;
-#if CL_RAGGED
-            const i64 key = kv0 + at;
-#else
-            const i64 key = pl_clamp(CL_ARG_INDICES[kv0 + at], 0, num_pages - 1);
-#endif
-            const elem_t* kr = reinterpret_cast<const elem_t*>(kbase + key * krow_bytes);
-            const elem_t* vr = reinterpret_cast<const elem_t*>(vbase + key * vrow_bytes);
-            float dot = 0.f;
-#pragma unroll
-            for (int i = 0; i < PL_KPANELS; ++i) dot += q[i] * to_f32(kr[64 * i + lane]);
-#pragma unroll
-            for (int b = 1; b < 64; b *= 2) dot += lane_xor(dot, lane, b);
-            const float score = (q_sign ? -dot : dot) * scale2;
-            if (pass == 0) {
-              top = fmaxf(top, score);
-            } else {
-              const float w = fast_exp2(score - top);
-              sum += w;
-#pragma unroll
-              for (int i = 0; i < PL_VPANELS; ++i) o[i] += w * to_f32(vr[64 * i + lane]);
-            }
-          }
-      if (PL_PART) {
-        const i64 prow = PL_PROW(split, m);
-#pragma unroll
-        for (int i = 0; i < PL_VPANELS; ++i) CL_ARG_PO[prow * CL_VDIM + 64 * i + lane] = o[i];
-        if (lane == 0) {
-          CL_ARG_PM[prow] = top;
-          CL_ARG_PL[prow] = sum;
-        }
-      } else {
-        const float inv = 1.0f / fmaxf(sum, 1.0e-30f);
-#pragma unroll
-        for (int i = 0; i < PL_VPANELS; ++i) CL_ARG_OUT[row * CL_VDIM + 64 * i + lane] = to_elem(o[i] * inv);
-#if CL_EMIT_LSE
-        if (lane == 0) CL_ARG_LSE[row] = cl_lse(top, sum);
-#endif
-      }
-    }
-    return;
-  }
-#endif
 
   // ---- each lane writes its rows' features (a row that saw no key: 0 and lse -inf) --------------
   // (row coordinates are worked out again from the lane number, behind a barrier for the
@@ -918,9 +771,9 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
     const float inv = 1.0f / fmaxf(l, 1.0e-30f);
 #endif
     const i64 orow = row_index(m);
-#if PL_PARTIALS
+#if CL_SPLITS > 1
     // split partials: unnormalised f32 values (16 bytes per lane and block), m and l by the g == 0 lanes
-    if (PL_PART) {
+    {
       const i64 prow = PL_PROW(split, m);
       float* dstp = CL_ARG_PO + prow * CL_VDIM + 4 * g_e;
 #pragma unroll
@@ -935,10 +788,8 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
 #endif
       }
       (void)inv;
-      continue;
     }
-#endif
-#if CL_SPLITS == 1
+#else
     pl_store_row<PL_FB, CL_DENSE>(CL_ARG_OUT + orow * CL_VDIM, acc[rt], inv, g_e);
 #if CL_EMIT_LSE
     if (g_e == 0) CL_ARG_LSE[orow] = cl_lse(m_run[rt], l);

@@ -236,7 +236,7 @@ def shared_ranges(spec: PagingSpec, head_dim: int) -> list:
     """Launch-time cuts: the number of ranges that the shared keys are cut into, and the table entries of an item of the requests' own.
 
     The workgroups of the shared keys come first and take part of the chip's 512 places, the own keys' fill the others and what falls
-    free.  A step of the former (32 keys, 128 rows) takes 0.62 us, and the own keys about 16 bytes of a place a ns: the former get the
+    free.  A step of the former (32 keys, 128 rows) takes 0.62 us, and the own keys about 16 bytes of a place a ns: the former get
     seven quarters of the share of the places that their work is of both (fewer end later than the own keys do), in ranges of two
     steps or more.  Partial and sum, us, f16, 64 requests of up to 1024 own keys behind 8192 by (ranges, pages an item): (4, 2) 58.7, (8, 2)
     46.6, (12, 2) 46.4, (16, 2) 48.7, (32, 2) 59.4, (8, 8) 53.1, (8, 16) 61.7; bf16, 200 of 700 behind 32768: (2, 2) 319, (4, 2) 200, (6, 2) 178,
