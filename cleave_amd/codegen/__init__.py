@@ -475,8 +475,12 @@ class HipCodeGen:
                 sig, entry, suffix = [names[op[f"{r}_COMBINE"]] for r in part_roles] + outs, COMBINE_ENTRY, "_COMBINE"
                 if plan.tiling.get("CHUNK_PAGES"):
                     sig = [names[op["INDPTR"]]] + sig
+                elif "QINDPTR" in op:
+                    sig = [names[op["QINDPTR"]]] + sig
             if plan.tiling.get("CHUNK_PAGES"):
                 unit.define("CL_CARG_INDPTR", op["INDPTR"])
+            elif "QINDPTR" in op:
+                unit.define("CL_CARG_QINDPTR", op["QINDPTR"])
             for r in part_roles:
                 unit.define(f"CL_CARG_{r}", op[r + suffix])
             unit.define("CL_CARG_OUT", op["OUT"])

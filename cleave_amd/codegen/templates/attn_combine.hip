@@ -5,7 +5,8 @@
 #define CL_CHUNK_PAGES 0
 #endif
 // CL_ITEM_RANGES: a run-time number of items that every request has first, one request's behind the other's.  With CL_OWN_CHUNK, the run-time
-// number of table entries of an item, items cut from the page table follow behind all of them.
+// number of table entries of an item, items cut from the page table follow behind all of them.  With CL_CARG_QINDPTR, the row pointers of
+// prompts, rows are query tokens, of which those ahead of the first request and behind the last have no items and stay as they are.
 #ifdef CL_ITEM_RANGES
 #define CB_FIXED_ITEMS 1
 #else
@@ -148,16 +149,24 @@ CL_COMBINE_NAME(CL_COMBINE_PARAMS) {
 #endif
     return nullptr;
   };
+  auto has_items = [&](const i64 row) {
+#ifdef CL_CARG_QINDPTR
+    return row >= (i64)CL_CARG_QINDPTR[0] * CL_Q_HEADS && row < (i64)CL_CARG_QINDPTR[batch] * CL_Q_HEADS;
+#else
+    return true;
+#endif
+  };
   if (gridDim.x == (unsigned)(CL_TOTAL_ROWS * (CL_VDIM / CB_COLS))) {       // (the launch's choice)
     const int group = threadIdx.x / CB_THREADS;
     const i64 row = (i64)blockIdx.x / (CL_VDIM / CB_COLS);
+    if (!has_items(row)) return;
     const int d = (int)(blockIdx.x % (CL_VDIM / CB_COLS)) * CB_COLS + 4 * (threadIdx.x % CB_THREADS);
     constexpr int PER_WAVE = 64 / CB_THREADS;
     add_up(CbTag<4>(), CbTag<CL_COMBINE_GROUPS>(), row, d, group, PER_WAVE - 1 - group % PER_WAVE);
     cb_finish(m, l, o, CL_CARG_OUT + row * CL_VDIM + d, lse(row, d));
   } else {
     const i64 idx = (i64)blockIdx.x * 256 + threadIdx.x, row = idx / (CL_VDIM / 4);
-    if (idx >= (i64)CL_TOTAL_ROWS * (CL_VDIM / 4)) return;
+    if (idx >= (i64)CL_TOTAL_ROWS * (CL_VDIM / 4) || !has_items(row)) return;
     const int d = (int)(idx % (CL_VDIM / 4)) * 4;
     add_up(CbTag<6>(), CbTag<1>(), row, d, 0, 0);
     cb_store(m, l, o, CL_CARG_OUT + row * CL_VDIM + d, lse(row, d));

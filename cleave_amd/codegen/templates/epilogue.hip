@@ -73,7 +73,7 @@ CL_DEVICE f32x4 ep_apply(f32x4 v, const elem_t* __restrict__ bias, const elem_t*
   return (f32x4){f[0], f[1], f[2], f[3]};
 }
 // The same in two halves, for wave tiles of many fragments: the pieces of bias and residual are asked for all at once, ahead of the
-// first use (fragment by fragment every one's wait was in sight: 4096 x 4096 x 1024 with a residual 42.5 us, RES_US this way, the bare
+// first use (fragment by fragment every wait was in sight: 4096 x 4096 x 1024 with a residual 42.5 us, 40.7 this way, the bare
 // product 32.1), and each fragment is finished with what has come.
 CL_DEVICE elem4 ep_piece(const elem_t* __restrict__ row, int n) {
   if constexpr (CL_N % 4 == 0) return *reinterpret_cast<const elem4*>(row + (n < CL_N ? n : CL_N - 4));
