@@ -9,7 +9,7 @@
 // and tile s + skip behind it.  A step is masked in a wave where one of its rows sees a part of the tile: at the causal end
 // (from n_full on) and where windows and sinks begin and end (before n_low).
 //
-// What bounds it: bf16, 32 / 8 heads, window 1024 + 4 sinks, packed prompts of 25263 tokens 537 us, 0.9 PFLOP/s of what is seen: no
+// What bounds it: bf16, 32 / 8 heads, window 1024 + 4 sinks, six packed prompts of 31433 tokens 505 us, 0.95 PFLOP/s of what is seen: no
 // one thing.  Without queries in and rows out 7 % less, without masks 7 %, without exponentials 10 %, without all of them 24 %;
 // the matrix unit is busy 45 % of the time and the clock is at the power cap.  Workgroups that stay and ask for their next
 // item's first tiles and queries ahead of their last one's stores were no faster (554 us against 551).
@@ -52,6 +52,44 @@ struct PwItem {          // all of it the same in every lane
   int ext, skip;         // keys that the last row may see; tiles between the sinks' and the first window's
   int first_step, n_steps, first_key;     // this range's steps; the first window's first key
 };
+// The request of an item: a request has as many items as its query tokens fill, counted up over the requests, 64 of them at a time
+// over the lanes of a wave.  (Items at the multiples of PW_QT packed tokens need no sum, but a request then has a part of one at either
+// end: half an item more of each request; and its bits
+// would depend on what is packed ahead of it.)
+struct PwRequest { int q0, q1, kv0, kv1, first_item; };
+CL_DEVICE int pw_running_sum(int x) {          // over the lanes of a wave, in order
+#define PW_ADD_FROM(CTRL, ROWS) x += __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false)
+  PW_ADD_FROM(0x111, 0xf);                     // of a row of 16 lanes, the lane 1, 2, 4 and 8 before
+  PW_ADD_FROM(0x112, 0xf);
+  PW_ADD_FROM(0x114, 0xf);
+  PW_ADD_FROM(0x118, 0xf);
+  PW_ADD_FROM(0x142, 0xa);                     // the last lane of rows 0 and 2 to the row behind each, of row 1 to rows 2 and 3
+  PW_ADD_FROM(0x143, 0xc);
+#undef PW_ADD_FROM
+  return x;
+}
+CL_DEVICE PwRequest pw_find_request(const int* __restrict__ q_ptr, int batch, int total_q, const int* __restrict__ kv_ptr, int n_idx, int item, int lane) {
+  PwRequest r = {0, 0, 0, 0, 0};               // (behind the last item: a request of nothing)
+  int before = 0;
+  for (int base = 0; base < batch; base += 64) {
+    const int b = base + lane < batch ? base + lane : batch - 1;
+    const int q0 = cl_clamp_ptr(q_ptr[b], total_q), q1 = cl_clamp_ptr(q_ptr[b + 1], total_q);
+    const int kv0 = cl_clamp_ptr(kv_ptr[b], n_idx), kv1 = cl_clamp_ptr(kv_ptr[b + 1], n_idx);
+    const int items = q1 > q0 && base + lane < batch ? (q1 - q0 + PW_QT - 1) / PW_QT : 0, sum = before + pw_running_sum(items);
+    const unsigned long long reached = __builtin_amdgcn_ballot_w64(sum > item);
+    if (reached) {
+      const int l = __builtin_ctzll(reached);
+      r.q0 = __builtin_amdgcn_readlane(q0, l);
+      r.q1 = __builtin_amdgcn_readlane(q1, l);
+      r.kv0 = __builtin_amdgcn_readlane(kv0, l);
+      r.kv1 = __builtin_amdgcn_readlane(kv1, l);
+      r.first_item = __builtin_amdgcn_readlane(sum - items, l);
+      return r;
+    }
+    before = __builtin_amdgcn_readlane(sum, 63);
+  }
+  return r;
+}
 // the tile of step s
 CL_DEVICE int pw_tile(const PwItem& it, int s) {
   s += it.first_step;
@@ -72,9 +110,9 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
   const i64 row_bytes = (i64)CL_KV_HEADS * CL_HEAD_DIM * 2;            // K, V: (key row, kv head, feature)
   const unsigned tiles_byte = (unsigned)(size_t)(__attribute__((address_space(3))) elem_t*)pw_tiles;
 
-  // ---- the item: a new one begins at every multiple of PW_QT packed query tokens and at every request boundary, item t = chunk w + request b
-  // for the one pair that overlaps; (range, kv head, item) in one order, of which XCD x walks the x-th eighth backwards: neighbouring
-  // items of a kv head, whose keys its L2 holds, later items of a request, which see more keys, first ------------------------
+  // ---- the item: requests one behind the other, each cut from its first query token on; (range, kv head, item) in one order, of
+  // which XCD x walks the x-th eighth backwards: neighbouring items of a kv head, whose keys its L2 holds, later items of a
+  // request, which see more keys, first ------------------------
   PwItem it;
   {
     // (XCD x is handed every eighth workgroup of a launch; the item axis is padded to a multiple of eight)
@@ -83,12 +121,11 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
     const int lin = all_items - 1 - (launch % 8 * (all_items / 8) + launch / 8), item = lin % gx;
     it.head = lin / gx % CL_KV_HEADS;
     it.split = lin / gx / CL_KV_HEADS;
-    const ClRequest found = cl_find_request(CL_ARG_QINDPTR, batch, total_q, PW_QT, 1, item, lane, CL_ARG_INDPTR, n_idx);
-    const int req = found.req, q0 = found.p0, q1 = found.p1, kv0 = found.s0, kv1 = found.s1;
-    const int chunk = item - req;
-    it.lo = q0 > chunk * PW_QT ? q0 : chunk * PW_QT;
-    const int hi = q1 < (chunk + 1) * PW_QT ? q1 : (chunk + 1) * PW_QT;
-    if (hi <= it.lo) return;                              // an index no (chunk, request) pair maps to
+    const PwRequest found = pw_find_request(CL_ARG_QINDPTR, batch, total_q, CL_ARG_INDPTR, n_idx, item, lane);
+    const int q1 = found.q1, kv0 = found.kv0, kv1 = found.kv1;
+    it.lo = found.q0 + (item - found.first_item) * PW_QT;
+    if (it.lo >= q1) return;                              // an index behind the last item
+    const int hi = q1 < it.lo + PW_QT ? q1 : it.lo + PW_QT;
     const int kv_len = kv1 > kv0 ? kv1 - kv0 : 0;
     it.kv0 = kv0;
     it.off = kv_len - q1;
@@ -227,7 +264,7 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
   n_low = __builtin_amdgcn_readfirstlane(n_low);
 
   // The values of masked steps times nothing: NaN from the first one on that is not finite.  (On the matrix cores, which have room:
-  // us, packed prompts of up to 8192 tokens, no check 533, this 545, dot products on the vector unit 548.)
+  // us, six packed prompts of 31433 tokens, no check 533, this 545, dot products on the vector unit 548.)
   f32x4 taint = (f32x4){0.f, 0.f, 0.f, 0.f};
   u32x4 no_bits = (u32x4){0u, 0u, 0u, 0u};
   const elem8 none = as_elem8(no_bits);

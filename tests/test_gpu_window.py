@@ -284,3 +284,17 @@ def test_compiled_prefill(ragged):
     assert not kernel.report.failures
     args = prefill_args(ragged, NEW, KEYS)
     check_prefill(kernel, args, prefill_want(args, ragged, NEW, KEYS, 60, 2))
+
+
+@pytest.mark.parametrize("ragged", [False, True], ids=["table", "packed"])
+def test_a_request_has_the_same_bits_in_any_company(ragged):
+    kernel = prefill_kernel(ragged, 60, 2, ranges=1)
+    args = prefill_args(ragged, NEW, KEYS)
+    out, lse = kernel(*args)
+    at_q, at_k = 0, 0
+    for n, m in zip(NEW, KEYS):
+        bounds = [torch.tensor([0, x], dtype=torch.int32, device="cuda") for x in (n, m)]
+        keys = [t[at_k:at_k + m] for t in args[1:3]] if ragged else args[1:3]
+        alone = kernel(args[0][at_q:at_q + n], *keys, *bounds, *([] if ragged else [args[5][at_k:at_k + m]]), args[-1])
+        assert torch.equal(alone[0], out[at_q:at_q + n]) and torch.equal(alone[1], lse[at_q:at_q + n])
+        at_q, at_k = at_q + n, at_k + m
