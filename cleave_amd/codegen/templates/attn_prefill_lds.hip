@@ -589,6 +589,28 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
   PL_WAITCNT(PL_VPANELS);
   pl_barrier();
   issue_k(3, 3 % PL_STAGES, PlC<0>{}, AllK{}, row3);
+#if CL_PREFIX
+  if (32 * wave >= n_rows) {
+    // a wave without rows: its share of the loads and the barriers of the bodies below, and no products, which slow down whoever runs
+    // beside it (us, bf16, 200 requests of 4 heads a kv head, whose last 128 rows are 32, behind 32768 keys 160.6 -> 158.3)
+    int slot = 0;
+    for (int step = 0;;) {
+      const int row_v = rows[0], row_k = fetched_row(step + 4);
+      rows[0] = rows[1];
+      rows[1] = row_k;
+      fetch_id(step + 5);
+      issue_v(step + 2, slot + 2 < PL_STAGES ? slot + 2 : slot + 2 - PL_STAGES, PlC<0>{}, AllV{}, row_v);
+      issue_k(step + 4, slot + 4 < 2 * PL_STAGES ? slot + 4 - PL_STAGES : slot + 4 - 2 * PL_STAGES, PlC<0>{}, AllK{}, row_k);
+      if (++step >= n_steps) break;
+      __builtin_amdgcn_sched_barrier(0);
+      PL_WAITCNT(PL_UNITS_PER);
+      pl_barrier();
+      slot = slot + 1 < PL_STAGES ? slot + 1 : 0;
+    }
+    PL_WAITCNT(0);
+    return;
+  }
+#endif
 
   // Body of step `step`, step % PL_STAGES == S.
   auto do_step = [&](auto s_c, const int step) __attribute__((always_inline)) {
