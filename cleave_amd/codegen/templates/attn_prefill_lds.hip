@@ -123,7 +123,10 @@
 // Images of K and of V: three, and four where the widest keys are read in two halves, the second out of an image still held, or
 // where three would let two workgroups onto a compute unit that 256 registers a wave do not hold (192 / 192 and 128 / 256 wide,
 // 32 heads x 2048 x 2048, us: three images and 40 / 146 spilled registers 177 / 357, four and none 105 / 117).
-#define PL_STAGES (CL_HEAD_DIM > 192 || CL_HEAD_DIM + CL_VDIM == 384 ? 4 : 3)
+// Loads are asked for one body earlier, into a fourth image, where others fill the memory beside them (us, f16, 64 requests of up to 1024 own
+// keys behind 8192 shared ones 45.0 -> 43.9, bf16, 200 of 700 behind 32768 164.7 -> 163.2).
+#define PL_AHEAD (CL_PREFIX && CL_HEAD_DIM <= 128)
+#define PL_STAGES (CL_HEAD_DIM > 192 || CL_HEAD_DIM + CL_VDIM == 384 ? 4 : 3 + PL_AHEAD)
 #define PL_ALONE (PL_STAGES * PL_STAGE * 4 > 163840)       // one workgroup of a compute unit: 512 registers a wave
 #define PL_KJ (CL_HEAD_DIM / 32)
 #define PL_FB (CL_VDIM / 16)
@@ -135,7 +138,7 @@ static_assert(PL_UNITS_PER < 16, "load counter range");
 
 __shared__ __attribute__((aligned(1024))) elem_t pl_tiles[PL_STAGES * PL_STAGE];
 #if !CL_RAGGED
-__shared__ __attribute__((aligned(256))) int pl_ids[2][4][64];   // table entries on their way in: [step parity][wave][lane]
+__shared__ __attribute__((aligned(256))) int pl_ids[2 + 2 * PL_AHEAD][4][64];   // table entries on their way in: [step][wave][lane]
 #endif
 
 #if CL_EMIT_PARTIAL
@@ -364,13 +367,14 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
   };
   // In the loop the lane's table entry travels like the tiles do, global -> LDS on the kernel's
   // own load counter, a step ahead of the loads that need it (a load the compiler tracks would
-  // make it wait for every load in flight): entry of step s into pl_ids[s & 1][wave][lane].
+  // make it wait for every load in flight): entry of step s into pl_ids[s % 2][wave][lane] (s % 4
+  // with PL_AHEAD).
   const unsigned ids_byte = (unsigned)(size_t)(__attribute__((address_space(3))) int*)&pl_ids[0][0][0];
   auto fetch_id = [&](int s) __attribute__((always_inline)) {
-    pl_dma4(PL_TABLE + PL_PAGE(kv0 + key_pos(s)), ids_byte + (unsigned)(((s & 1) * 4 + wave) * 256));
+    pl_dma4(PL_TABLE + PL_PAGE(kv0 + key_pos(s)), ids_byte + (unsigned)(((s & (1 + 2 * PL_AHEAD)) * 4 + wave) * 256));
   };
   auto fetched_row = [&](int s) __attribute__((always_inline)) {
-    return PL_ROW(pl_clamp(pl_ids[s & 1][wave][lane], 0, num_pages - 1), kv0 + key_pos(s));
+    return PL_ROW(pl_clamp(pl_ids[s & (1 + 2 * PL_AHEAD)][wave][lane], 0, num_pages - 1), kv0 + key_pos(s));
   };
 #endif
 
@@ -380,20 +384,25 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
   using AllV = PlC<PL_VPANELS>;
   int rows[2] = {0, 0};                        // table form: the lane's key rows of V of the next two bodies
 #if CL_RAGGED
-  constexpr int row0 = 0, row1 = 0, row3 = 0;
+  constexpr int row0 = 0, row1 = 0, row2 = 0, row3 = 0;
 #else
-  const int row0 = row_of(0), row1 = row_of(1), row3 = row_of(3);
-  rows[0] = row_of(2);
-  rows[1] = row3;
+  const int row0 = row_of(0), row1 = row_of(1), row2 = row_of(2), row3 = row_of(3);
+  rows[0] = PL_AHEAD ? row3 : row2;
+  rows[1] = PL_AHEAD ? row_of(4) : row3;
 #endif
   issue_k(0, 0, PlC<0>{}, AllK{}, row0);
   issue_k(1, 1, PlC<0>{}, AllK{}, row1);
   issue_v(0, 0, PlC<0>{}, AllV{}, row0);
-  issue_k(2, 2, PlC<0>{}, AllK{}, rows[0]);
+  issue_k(2, 2, PlC<0>{}, AllK{}, row2);
 #if !CL_RAGGED
-  fetch_id(4);
+  fetch_id(4 + PL_AHEAD);
+  if constexpr (PL_AHEAD) fetch_id(6);
 #endif
   issue_v(1, 1, PlC<0>{}, AllV{}, row1);
+  if constexpr (PL_AHEAD) {
+    issue_k(3, 3, PlC<0>{}, AllK{}, row3);
+    issue_v(2, 2, PlC<0>{}, AllV{}, row2);
+  }
 
   // Query rows as the B operand: lane (c, g) holds Q[row][32 j + 8 g .. +8]; padded rows are 0.
   elem8 qf[2][PL_KJ];
@@ -565,7 +574,7 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
     for (int i = 1; i < 8; ++i) v = fmaxf(v, sc[i >> 2][i & 3]);
     return v;
   };
-  PL_WAITCNT(PL_KPANELS + 2 * PL_VPANELS + !CL_RAGGED);
+  PL_WAITCNT(PL_KPANELS + 2 * PL_VPANELS + (1 + PL_AHEAD) * !CL_RAGGED + PL_AHEAD * PL_UNITS_PER);
   pl_barrier();
 #pragma unroll
   for (int j0 = 0; j0 < PL_KJ; j0 += KH) {
@@ -586,24 +595,24 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
   }
 #endif
   // the images of body 0 (V 0, K 2) have landed; K 0 has been read by everybody
-  PL_WAITCNT(PL_VPANELS);
+  PL_WAITCNT(PL_VPANELS + PL_AHEAD * PL_UNITS_PER);
   pl_barrier();
-  issue_k(3, 3 % PL_STAGES, PlC<0>{}, AllK{}, row3);
+  issue_k(3 + PL_AHEAD, (3 + PL_AHEAD) % PL_STAGES, PlC<0>{}, AllK{}, PL_AHEAD ? rows[1] : row3);
 #if CL_PREFIX
   if (32 * wave >= n_rows) {
     // a wave without rows: its share of the loads and the barriers of the bodies below, and no products, which slow down whoever runs
     // beside it (us, bf16, 200 requests of 4 heads a kv head, whose last 128 rows are 32, behind 32768 keys 160.6 -> 158.3)
     int slot = 0;
     for (int step = 0;;) {
-      const int row_v = rows[0], row_k = fetched_row(step + 4);
+      const int row_v = rows[0], row_k = fetched_row(step + 4 + PL_AHEAD);
       rows[0] = rows[1];
       rows[1] = row_k;
-      fetch_id(step + 5);
-      issue_v(step + 2, slot + 2 < PL_STAGES ? slot + 2 : slot + 2 - PL_STAGES, PlC<0>{}, AllV{}, row_v);
-      issue_k(step + 4, slot + 4 < 2 * PL_STAGES ? slot + 4 - PL_STAGES : slot + 4 - 2 * PL_STAGES, PlC<0>{}, AllK{}, row_k);
+      fetch_id(step + 5 + 2 * PL_AHEAD);
+      issue_v(step + 2 + PL_AHEAD, (slot + 2 + PL_AHEAD) % PL_STAGES, PlC<0>{}, AllV{}, row_v);
+      issue_k(step + 4 + PL_AHEAD, (slot + 4 + PL_AHEAD) % PL_STAGES, PlC<0>{}, AllK{}, row_k);
       if (++step >= n_steps) break;
       __builtin_amdgcn_sched_barrier(0);
-      PL_WAITCNT(PL_UNITS_PER);
+      PL_WAITCNT((1 + PL_AHEAD) * PL_UNITS_PER + PL_AHEAD);
       pl_barrier();
       slot = slot + 1 < PL_STAGES ? slot + 1 : 0;
     }
@@ -619,20 +628,21 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
 #if CL_RAGGED
     constexpr int row_v = 0, row_k = 0;
 #else
+    // (with PL_AHEAD every step below is one later, and entries are asked for two bodies ahead)
     // (V of step + 2, whose row was looked up two bodies ago; K of step + 4, whose entry was asked for in the last body
     // ahead of the loads that the wait before this one left out)
-    const int row_v = rows[0], row_k = fetched_row(step + 4);
+    const int row_v = rows[0], row_k = fetched_row(step + 4 + PL_AHEAD);
     rows[0] = rows[1];
     rows[1] = row_k;
-    fetch_id(step + 5);
+    fetch_id(step + 5 + 2 * PL_AHEAD);
 #endif
     // the loads of this body, in four shares between its matrix work (a wave stands still while a load waits for the path
     // into the compute unit): V of step + 2, K of step + 4
     auto ask = [&](auto place_c) __attribute__((always_inline)) {
       constexpr int LO = decltype(place_c)::value * PL_UNITS_PER / 4, HI = (decltype(place_c)::value + 1) * PL_UNITS_PER / 4;
       constexpr int VL = LO < PL_VPANELS ? LO : PL_VPANELS, VH = HI < PL_VPANELS ? HI : PL_VPANELS;
-      issue_v(step + 2, (S + 2) % PL_STAGES, PlC<VL>{}, PlC<VH>{}, row_v);
-      issue_k(step + 4, (S + 4) % PL_STAGES, PlC<LO - VL>{}, PlC<HI - VH>{}, row_k);
+      issue_v(step + 2 + PL_AHEAD, (S + 2 + PL_AHEAD) % PL_STAGES, PlC<VL>{}, PlC<VH>{}, row_v);
+      issue_k(step + 4 + PL_AHEAD, (S + 4 + PL_AHEAD) % PL_STAGES, PlC<LO - VL>{}, PlC<HI - VH>{}, row_k);
     };
     __builtin_amdgcn_sched_barrier(0);
     if (step >= n_full) mask(st, step);
@@ -744,7 +754,7 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
   // it reads ahead), and the images that the last body read last are free for what the next one asks for.
   auto turn = [&]() __attribute__((always_inline)) {
     __builtin_amdgcn_sched_barrier(0);
-    PL_WAITCNT(PL_UNITS_PER);
+    PL_WAITCNT((1 + PL_AHEAD) * PL_UNITS_PER + PL_AHEAD);
     pl_barrier();
   };
 
