@@ -238,10 +238,10 @@ def shared_ranges(spec: PagingSpec, head_dim: int) -> list:
     The workgroups of the shared keys come first and take part of the chip's 512 places, the own keys' fill the others and what falls
     free.  A step of the former (32 keys, 128 rows) takes 0.62 us, and the own keys about 16 bytes of a place a ns: the former get
     seven quarters of the share of the places that their work is of both (fewer end later than the own keys do), in ranges of two
-    steps or more.  Partial and sum, us, f16, 64 requests of up to 1024 own keys behind 8192 by (ranges, pages an item): (4, 2) 58.7, (8, 2)
-    46.6, (12, 2) 46.4, (16, 2) 48.7, (32, 2) 59.4, (8, 8) 53.1, (8, 16) 61.7; bf16, 200 of 700 behind 32768: (2, 2) 319, (4, 2) 200, (6, 2) 178,
-    (7, 2) 172, (9, 2) 180, (18, 2) 190.  Own keys ahead of the shared ones 53.7 and 188, both kinds in turn 49.2 and 222: a compute unit's shared keys
-    then wait for their loads behind its own keys'.  Items: as many workgroups as give every place two, of a step or more."""
+    steps or more.  us, f16, 64 requests of up to 1024 own keys behind 8192, by ranges, two pages an item: 6 49.2, 8 44.4, 9 43.9, 12 43.8,
+    16 46.6; bf16, 200 of 700 behind 32768, three pages: 5 192, 6 170, 7 164, 8 163, 9 169, 13 172.  Own keys ahead of the shared ones 55 and
+    184, both kinds in turn 49 and 222, 256 workgroups of the shared keys, the own keys, then the others 44 and 174: a compute unit's shared
+    keys wait for their loads behind its own keys'.  Items: as many workgroups as give every place two, of a step or more."""
     from ...core.target import current_target
 
     places = 2 * current_target().arch.compute_units
