@@ -149,9 +149,12 @@ CL_COMBINE_NAME(CL_COMBINE_PARAMS) {
 #endif
     return nullptr;
   };
+#ifdef CL_CARG_QINDPTR
+  const int first_token = CL_CARG_QINDPTR[0], end_token = CL_CARG_QINDPTR[batch];      // (on their way beside the partials)
+#endif
   auto has_items = [&](const i64 row) {
 #ifdef CL_CARG_QINDPTR
-    return row >= (i64)CL_CARG_QINDPTR[0] * CL_Q_HEADS && row < (i64)CL_CARG_QINDPTR[batch] * CL_Q_HEADS;
+    return row >= (i64)first_token * CL_Q_HEADS && row < (i64)end_token * CL_Q_HEADS;
 #else
     return true;
 #endif
@@ -159,17 +162,17 @@ CL_COMBINE_NAME(CL_COMBINE_PARAMS) {
   if (gridDim.x == (unsigned)(CL_TOTAL_ROWS * (CL_VDIM / CB_COLS))) {       // (the launch's choice)
     const int group = threadIdx.x / CB_THREADS;
     const i64 row = (i64)blockIdx.x / (CL_VDIM / CB_COLS);
-    if (!has_items(row)) return;
     const int d = (int)(blockIdx.x % (CL_VDIM / CB_COLS)) * CB_COLS + 4 * (threadIdx.x % CB_THREADS);
     constexpr int PER_WAVE = 64 / CB_THREADS;
     add_up(CbTag<4>(), CbTag<CL_COMBINE_GROUPS>(), row, d, group, PER_WAVE - 1 - group % PER_WAVE);
+    if (!has_items(row)) return;
     cb_finish(m, l, o, CL_CARG_OUT + row * CL_VDIM + d, lse(row, d));
   } else {
     const i64 idx = (i64)blockIdx.x * 256 + threadIdx.x, row = idx / (CL_VDIM / 4);
-    if (idx >= (i64)CL_TOTAL_ROWS * (CL_VDIM / 4) || !has_items(row)) return;
+    if (idx >= (i64)CL_TOTAL_ROWS * (CL_VDIM / 4)) return;
     const int d = (int)(idx % (CL_VDIM / 4)) * 4;
     add_up(CbTag<6>(), CbTag<1>(), row, d, 0, 0);
-    cb_store(m, l, o, CL_CARG_OUT + row * CL_VDIM + d, lse(row, d));
+    if (has_items(row)) cb_store(m, l, o, CL_CARG_OUT + row * CL_VDIM + d, lse(row, d));
   }
 }
 #elif CL_SPLITS > 1 && CL_EMIT_COMBINE && CL_PO_ELEM

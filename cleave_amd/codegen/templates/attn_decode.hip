@@ -339,7 +339,7 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
   const int hi = p1 > lo ? p1 : lo;
 #endif
   u.pages = CL_ARG_INDICES + lo;
-  u.n_pages = hi - lo;
+  u.n_pages = num_pages > 0 ? hi - lo : 0;            // (a cache without rows has no keys, whatever the table says)
   u.pool_pages = num_pages;
   u.page_reg = 0;
   {
@@ -365,7 +365,7 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
   // sum is clamped to the pages the request owns.
   const int req = unit / CL_KV_HEADS, head = unit % CL_KV_HEADS;
 #if CL_WINDOW
-  const int p0 = cl_clamp_ptr(CL_ARG_INDPTR[req], n_idx), p1 = cl_clamp_ptr(CL_ARG_INDPTR[req + 1], n_idx);
+  const int p0 = cl_clamp_ptr(CL_ARG_INDPTR[req], n_idx), p1 = num_pages > 0 ? cl_clamp_ptr(CL_ARG_INDPTR[req + 1], n_idx) : p0;
 #else
   const int p0 = CL_ARG_INDPTR[req], p1 = CL_ARG_INDPTR[req + 1];
 #endif

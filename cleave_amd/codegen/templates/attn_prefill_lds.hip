@@ -184,7 +184,7 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
 #if CL_PREFIX
   const int lo = item * PL_ROWS;
   const int n_rows = batch * PL_GROUP - lo < PL_ROWS ? batch * PL_GROUP - lo : PL_ROWS;
-  const int all_keys = n_shared * CL_PAGE_SIZE;
+  const int all_keys = num_pages > 0 ? n_shared * CL_PAGE_SIZE : 0;
   const int per_range = ((all_keys + PL_STEP - 1) / PL_STEP + prefix_ranges - 1) / prefix_ranges * PL_STEP;
   const int kv0 = split * per_range;                    // this range's first key
   int n_keys = all_keys - kv0 < per_range ? all_keys - kv0 : per_range;

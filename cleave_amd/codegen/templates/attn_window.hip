@@ -126,7 +126,11 @@ CL_PARTIAL_NAME(CL_PARTIAL_PARAMS) {
     it.lo = found.q0 + (item - found.first_item) * PW_QT;
     if (it.lo >= q1) return;                              // an index behind the last item
     const int hi = q1 < it.lo + PW_QT ? q1 : it.lo + PW_QT;
+#if CL_RAGGED
     const int kv_len = kv1 > kv0 ? kv1 - kv0 : 0;
+#else
+    const int kv_len = kv1 > kv0 && num_pages > 0 ? kv1 - kv0 : 0;
+#endif
     it.kv0 = kv0;
     it.off = kv_len - q1;
     it.n_rows = (hi - it.lo) * PW_GROUP;

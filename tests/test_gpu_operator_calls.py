@@ -106,6 +106,19 @@ def test_empty_batches():
         assert out.shape[0] == 0 and lse.shape[0] == 0
 
 
+def test_caches_without_rows():
+    """Whatever a table says, a cache of no pages holds no keys: zeros and -inf, and nothing is read."""
+    for kernel, args in ((W.decode_kernel(16, 100, 4, split=2, ranges=3), W.decode_args(DECODE_LENS, 16)),
+                         (W.decode_kernel(16, 100, 4, split=8), W.decode_args(DECODE_LENS, 16)), (W.decode_kernel(1, 100, 4), W.decode_args(DECODE_LENS, 1)),
+                         (W.prefill_kernel(False, 60, 2, ranges=1), W.prefill_args(False, W.NEW, W.KEYS)),
+                         (W.prefill_kernel(False, 60, 2, ranges=3), W.prefill_args(False, W.NEW, W.KEYS)),
+                         (S.shared_kernel(16), S.shared_args(40, DECODE_LENS, 16)), (S.shared_kernel(1), S.shared_args(40, DECODE_LENS, 1))):
+        args[1], args[2] = (t[:0].clone() for t in args[1:3])
+        out, lse = kernel(*args)
+        torch.cuda.synchronize()
+        assert bool((out == 0).all()) and bool((lse == -torch.inf).all())
+
+
 @pytest.mark.parametrize("ranges", [1, 2])
 def test_prompts_of_many_requests(ranges):
     new = [(7 * i) % 5 * (i % 3) for i in range(300)]                        # more requests than a search reads at once, many without tokens
