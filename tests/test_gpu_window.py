@@ -66,16 +66,14 @@ def check_decode(kernel, args, lens, page, window, sinks):
 LENS = [1, 5, 31, 32, 33, 64, 65, 100, 0, 333, 129, 1000]
 
 
-@pytest.mark.parametrize("page", [1, 16, 64])
-@pytest.mark.parametrize("split", [None, 8])
+@pytest.mark.parametrize("page,split", [(1, None), (64, None), (1, 8), (16, 8)])
 @pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (31, 0), (32, 4), (33, 32), (64, 33), (100, 100), (97, 1), (2000, 4), (40, 400)])
 def test_decode(page, split, window, sinks):
     print(f"window decode page={page} split={split} window={window} sinks={sinks}", flush=True)
     check_decode(decode_kernel(page, window, sinks, split=split), decode_args(LENS, page), LENS, page, window, sinks)
 
 
-@pytest.mark.parametrize("page", [1, 16, 64])
-@pytest.mark.parametrize("ranges", [-1, 1, 5])
+@pytest.mark.parametrize("page,ranges", [(1, -1), (64, -1), (16, 1), (64, 5)])
 @pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (31, 0), (32, 4), (33, 32), (64, 33), (100, 100), (97, 1), (2000, 4), (40, 400)])
 def test_decode_by_items(page, ranges, window, sinks):
     """What is seen in equal parts by workgroups of one wave per kv head; more parts than steps leave some empty."""
@@ -197,8 +195,7 @@ NEW = [1, 4, 5, 33, 0, 64, 7, 130, 300]
 KEYS = [1, 40, 5, 33, 9, 200, 3, 130, 1000]      # equal, cached keys, no queries, fewer keys than queries
 
 
-@pytest.mark.parametrize("ragged", [False, True], ids=["table", "packed"])
-@pytest.mark.parametrize("ranges", [-1, 1, 2, 7])
+@pytest.mark.parametrize("ragged,ranges", [(False, -1), (True, -1), (False, 1), (True, 1), (False, 7), (True, 2)])
 @pytest.mark.parametrize("window,sinks", [(1, 0), (1, 2), (31, 0), (32, 4), (33, 32), (64, 33), (100, 0), (97, 100), (5000, 4), (40, 500)])
 def test_prefill(ragged, ranges, window, sinks):
     print(f"window prefill ragged={ragged} ranges={ranges} window={window} sinks={sinks}", flush=True)
