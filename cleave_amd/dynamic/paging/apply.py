@@ -238,10 +238,13 @@ def shared_ranges(spec: PagingSpec, head_dim: int) -> list:
     The workgroups of the shared keys come first and take part of the chip's 512 places, the own keys' fill the others and what falls
     free.  A step of the former (32 keys, 128 rows) takes 0.62 us, and the own keys about 16 bytes of a place a ns: the former get
     seven quarters of the share of the places that their work is of both (fewer end later than the own keys do), in ranges of two
-    steps or more.  us, f16, 64 requests of up to 1024 own keys behind 8192, by ranges, two pages an item: 6 49.2, 8 44.4, 9 43.9, 12 43.8,
-    16 46.6; bf16, 200 of 700 behind 32768, three pages: 5 192, 6 170, 7 164, 8 163, 9 169, 13 172.  Own keys ahead of the shared ones 55 and
-    184, both kinds in turn 49 and 222, 256 workgroups of the shared keys, the own keys, then the others 44 and 174: a compute unit's shared
-    keys wait for their loads behind its own keys'.  Items: as many workgroups as give every place two, of a step or more."""
+    steps or more.  Nor more than pay for their partials, which cost a range the time of so and so many steps: about the root of
+    ``room``, what all steps and a range's partials take by one another.  us by ranges: f16, 64 requests of up to 1024 own keys behind 8192
+    6 49.2, 8 44.4, 9 43.9, 12 43.8, 16 46.6; bf16, 200 of 700 behind 32768 5 192, 6 170, 7 164, 8 163, 9 169, 13 172; requests of few own
+    keys, 35 behind 1892 4 19.2, 8 17.0, 16 17.6, 28 20.5, 128 behind 8192 4 45.6, 8 32.1, 16 37.6, 16 behind 8192 12 20.5, 24 17.1, 64 21.8;
+    200 of 100 to 500 behind 2048 1 71.6, 2 66.9, 4 72.7.  Own keys ahead of the shared ones 55 (the first) and 184 (the second), both kinds in
+    turn 49 and 222, 256 workgroups of the shared keys, the own keys, then the others 44 and 174: a compute unit's shared keys wait for their
+    loads behind its own keys'.  Items: as many workgroups as give every place two, of whole steps."""
     from ...core.target import current_target
 
     places = 2 * current_target().arch.compute_units
@@ -250,10 +253,14 @@ def shared_ranges(spec: PagingSpec, head_dim: int) -> list:
     pairs = f"({spec.num_kv_heads} * max(1, ceildiv({b} * {spec.group}, 128)))"            # (kv head, 128 rows)
     shared = f"({pairs} * {steps})"
     own = f"({spec.index_dim} * {page} * {spec.num_kv_heads * head_dim} // 1766)"           # in steps of the former
-    prefix = f"max(1, min({steps} // 2, {places} // {pairs}, {places * 7 // 4} * {shared} // max(1, {shared} + {own}) // {pairs}))"
+    room = f"({steps} * 200000 // max(1, {b} * {spec.num_qo_heads * (head_dim + 2)}))"
+    best = " + ".join(["1", *(f"{more} * min(1, {room} // {least})" for more, least in (
+        (1, 3), (1, 8), (1, 15), (2, 32), (2, 60), (4, 130), (4, 240), (8, 540), (8, 1000), (16, 2250), (16, 4000)))])
+    prefix = f"max(1, min({steps} // 2, {places} // {pairs}, ceildiv({places * 7 // 4} * {shared} // max(1, {shared} + {own}), {pairs}), {best}))"
     pieces = -(-spec.num_kv_heads // 4) * -(-spec.group // 16)                               # workgroups of an item
     most = max(1, MAX_CHUNK_TOKENS // page)
-    chunk = f"max({-(-KV_STEP // page)}, min({most}, ceildiv({spec.index_dim} * {pieces}, {2 * places})))"
+    step = -(-KV_STEP // page)                                                               # table entries of a step
+    chunk = f"max({step}, min({most}, ceildiv({spec.index_dim} * {pieces}, {2 * places * step}) * {step}))"
     return [("prefix_ranges", prefix), ("own_chunk", chunk)]
 
 
@@ -328,9 +335,10 @@ def prefill_ranges_expr(spec: PagingSpec, head_dim: int, ranges: int = -1) -> st
     """The launch-time number of ranges that an item's keys of a window are dealt out to: the fixed value, or for -1 by what more of them
     save and cost.  ``r`` ranges save 1 - 1 / r of an item's steps (0.62 us each) and cost a launch and ``r`` times the partials, which are
     written and read at 3 TB/s: with ``room`` the quotient of the former's steps and the latter's bytes the best number is its root, taken
-    in steps of one, two, four and eight; no more than give every compute unit two workgroups and a range eight steps.  us, bf16, 32 / 8
-    heads, table, window and new tokens by ranges: 4000, 1 x 8 tokens 1 76.1, 4 26.3, 8 22.3, 16 18.4; 1 x 40 1 77.7, 4 29.5, 8 28.4, 16 26.7;
-    2 x 300 1 79.4, 2 70.8, 4 70.7, 8 89.7; 1000, 2 x 300 1 29.8, 2 36.2; 500, 1 x 100 1 18.0, 2 17.3, 8 22.9; packed, 4096, 1 x 2000 1 49.5, 2 70.8."""
+    in steps of one, two, four and eight; no more than give every compute unit two workgroups and a range three steps.  us, bf16, 32 / 8
+    heads, table, window and new tokens by ranges: 4000, 1 x 8 tokens 1 75.3, 4 26.4, 8 18.2, 16 14.2; 1 x 40 1 78.3, 4 29.5, 8 23.0, 16 21.9;
+    2 x 300 1 79.9, 2 69.6, 4 68.4, 8 80.6; 1000, 2 x 300 1 28.7, 2 36.5; 500, 1 x 100 1 16.6, 2 16.4, 8 20.5; 300, 2 x 8 1 11.6, 4 9.4, 8 9.8; packed,
+    4096, 1 x 2000 1 47.2, 2 65.7."""
     from ...core.target import current_target
 
     if ranges > 0:
@@ -342,7 +350,7 @@ def prefill_ranges_expr(spec: PagingSpec, head_dim: int, ranges: int = -1) -> st
     room = f"({steps} * 232500 // max(1, {spec.tokens_dim} * {spec.num_qo_heads * (head_dim + 2)}))"
     best = f"1 + min(1, {room} // 6) + min(1, {room} // 12) + 2 * min(1, {room} // 24) + 4 * min(1, {room} // 80) + 8 * min(1, {room} // 300)"
     items = f"(ceildiv({spec.tokens_dim}, {tokens}) + batch)"
-    return f"max(1, min({2 * current_target().arch.compute_units} // max(1, {items} * {spec.num_kv_heads}), min({steps} // 8, {best})))"
+    return f"max(1, min({2 * current_target().arch.compute_units} // max(1, {items} * {spec.num_kv_heads}), min({steps} // 3, {best})))"
 
 
 def _prefill_plan(spec: PagingSpec, dense: DenseAttention, shared: bool | None = None, knobs=None, ranges: int = -1) -> KernelPlan:
