@@ -48,6 +48,8 @@
 //                kv head, CL_WAVES of them a workgroup; a window's are `ranges` (a run-time argument) equal parts of what each
 //                request sees.  The cache rows of an item's tokens are worked out once, into LDS: unseen tokens of its ragged
 //                steps repeat a seen one there.
+//                HBM bounds a window's items where requests are many: f16, 32 / 8 heads, pages of 64, 64 requests that see up to 4160 keys
+//                175 us, 5.8 TB/s (the single kernel 276); one request is two launches of dependent loads, window 1000 9.0 us.
 
 #define ATT_RAISE_BY 8.0f
 #ifndef CL_OWN_PART
