@@ -7,6 +7,7 @@
 //   own keys     read by their request alone (att_own_part, attn_decode.hip: registers, nothing through LDS on the way in);
 //   partials     of `prefix_ranges` ranges of the shared keys (request, range, query head[, d]) and, behind them, of items of
 //                `own_chunk` entries of the requests' own table (item, query head[, d]), f32, merged by attn_combine.hip.
+// Partials are f32; weights are rounded to the element type for either kind's value product, as the matrix cores take it, and summed before.
 // Read by every request for itself, the shared keys would be `batch` times the traffic.
 //
 // One launch holds both kinds: the first part is bound by the matrix cores or L2, the second by HBM, and their workgroups run beside

@@ -5,6 +5,9 @@
 // reference points raised only by weights that outgrow them) are those of attn_prefill_lds.hip: an item is 128 rows (PW_QT
 // consecutive query tokens x the head group) of one request and kv head, four waves of 32 rows share every 32-key step of K and V.
 //
+// Scores, reference points, sums and outputs are f32.  Weights are rounded to the element type for the value product, as the matrix cores
+// take it (half a step of a weight each, together at most about that of the result); their sum is taken before.
+//
 // Steps are numbered without the key tiles that no row of an item sees: step s is tile s of the request up to the sinks' last tile
 // and tile s + skip behind it.  A step is masked in a wave where one of its rows sees a part of the tile: at the causal end
 // (from n_full on) and where windows and sinks begin and end (before n_low).
