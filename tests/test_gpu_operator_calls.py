@@ -203,3 +203,21 @@ def test_prompts_past_32_bits():
         torch.cuda.synchronize()
         same(out, want, tol, "out")
         same(lse, want_lse, lse_tol, "lse")
+
+
+@pytest.mark.parametrize("hq,hkv", [(4, 2), (32, 2), (32, 16), (64, 4)])
+def test_head_layouts(hq, hkv):
+    """Groups of two and of 16, more kv heads than a workgroup has waves."""
+    lens = [70, 0, 1, 333]
+    args = W.decode_args(lens, 16, hq=hq, hkv=hkv)
+    for form in (dict(), dict(split=4), dict(split=2, ranges=-1), dict(split=2, ranges=3, waves=min(hkv, 8))):
+        print(f"head layouts {hq}/{hkv} decode {form}", flush=True)
+        W.check_decode(W.decode_kernel(16, 50, 3, hq=hq, hkv=hkv, **{"waves": min(hkv, 8) if form.get("ranges") else 4, **form}), args, lens, 16, 50, 3)
+    for ragged in (False, True):
+        for ranges in (1, 3):
+            print(f"head layouts {hq}/{hkv} prompts ragged={ragged} ranges={ranges}", flush=True)
+            args = W.prefill_args(ragged, W.NEW, W.KEYS, hq=hq, hkv=hkv)
+            W.check_prefill(W.prefill_kernel(ragged, 60, 2, hq=hq, hkv=hkv, ranges=ranges), args, W.prefill_want(args, ragged, W.NEW, W.KEYS, 60, 2))
+    for page in (1, 16):
+        print(f"head layouts {hq}/{hkv} shared page={page}", flush=True)
+        S.check(S.shared_kernel(page, hq=hq, hkv=hkv), S.shared_args(20, lens, page, hq=hq, hkv=hkv), lens, page)
